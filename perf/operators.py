@@ -323,7 +323,8 @@ def run(state):
         g = state["g"].double()
         norm = torch.sqrt((g * g).sum())
         norm = norm if state["unscale"] is None else norm * state["unscale"].double()
-        scale = torch.where(norm < MAX_NORM, 1.0, MAX_NORM / norm)
+        scale = torch.where(norm < MAX_NORM, 1.0, MAX_NORM / norm)  # the factor that the step applies to the gradient
+        scale = scale if state["unscale"] is None else scale * state["unscale"].double()
         return torch.stack([norm, torch.where(torch.isfinite(norm), scale, math.nan)]).float()
     elif op == "adamw32":
         tid, off, valid = _per_element(state, state["starts"], state["total"])
@@ -403,7 +404,8 @@ def exact(case, seed):
     if case["op"] == "norm":
         total = sum((part.double() ** 2).sum() for part in s["g"].split(1 << 24))
         norm = total.sqrt() * (1.0 if s["unscale"] is None else float(s["unscale"]))
-        return torch.stack([norm, torch.clamp(MAX_NORM / norm, max=1.0)])
+        factor = torch.clamp(MAX_NORM / norm, max=1.0) * (1.0 if s["unscale"] is None else float(s["unscale"]))
+        return torch.stack([norm, factor])
     eight = case["op"] == "adamw8"
     dev = s["p"].device
     t = s["count0"] + 1
