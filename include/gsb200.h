@@ -525,6 +525,116 @@ GS_API int gs_adam_step_flat_device(float* params, const float* grads, float* mu
                                     float lr, double b1, double b2, double eps, int32_t* state,
                                     gs_stream_t stream);
 
+/* ---- AdamW over many tensors ----------------------------------------- */
+
+/*
+ * No reference counterpart (the reference's optimizers are optax.adam over
+ * fixed groups): AdamW with decoupled weight decay as optax.adamw defines it,
+ * over any number of tensors of any sizes in one launch per 256 of them.
+ * With c = state[0] before the call, t = c + 1 and s = *grad_scale (1 if
+ * NULL), for every element of every tensor:
+ *   g  = s grad;  m' = b1 m + (1 - b1) g;  v' = b2 v + (1 - b2) g^2
+ *   lr = lr_init decay_rate ^ (c / transition_steps)
+ *   param -= lr (m' / (1 - b1^t) / (sqrt(v' / (1 - b2^t)) + eps)
+ *                + weight_decay param)
+ * in fp32. Elements whose active flag is 0 keep their parameter (their
+ * moments are updated, as by gs_adam_step). copy, if set, receives the
+ * parameter rounded to copy_type. The call leaves c + 1 in state[0]; if s is
+ * not finite it changes nothing but state[2], which it increments.
+ */
+#define GS_TYPE_F32 0
+#define GS_TYPE_BF16 1
+#define GS_TYPE_F16 2
+/* Elements of a block of 8-bit moments. */
+#define GS_ADAMW_BLOCK 128
+
+typedef struct GsAdamwTensor {
+  float* param;
+  const void* grad;      /* count values of grad_type */
+  void* mu;              /* moment_bits 32: count floats; 8: count codes */
+  void* nu;
+  uint8_t* mu_exp;       /* moment_bits 8: ceil(count / 128) exponent bytes */
+  uint8_t* nu_exp;
+  void* copy;            /* nullable: count values of copy_type (not F32) */
+  const uint8_t* active; /* nullable: count / width flags, flag r for elements
+                            [r width, (r + 1) width) */
+  int64_t count;         /* >= 0, at most 2^37 */
+  int32_t width;         /* 1 .. 65535; read where active is set */
+  int32_t grad_type;
+  int32_t copy_type;     /* read where copy is set */
+  float lr_init, decay_rate, transition_steps, weight_decay;
+  int32_t reserved;
+} GsAdamwTensor;
+
+typedef struct GsAdamwConfig {
+  double b1, b2;        /* in [0, 1) */
+  double eps;           /* > 0, also as a float */
+  int32_t moment_bits;  /* 32 or 8 */
+  uint32_t seed;        /* moment_bits 8: of the stochastic rounding */
+} GsAdamwConfig;
+
+/*
+ * tensors and config are read on the host at call time. grad_scale (device,
+ * nullable) is read by the kernel. state: device int32[4], [count, ticket
+ * used internally, steps skipped, 0], zeroed by the caller at the start (or
+ * count set). The tensors' parameters, moments and copies must not overlap.
+ * Everything is ordered on `stream`; with the count and grad_scale on the
+ * device a captured CUDA graph replays successive steps.
+ *
+ * 8-bit moments: the tensor's elements in blocks of 128, the last one partial.
+ * Each moment has one exponent byte F per block: its codes stand for
+ * multiples of 2^(F - 127), as mu: sign, 4-bit exponent, 3-bit mantissa (top
+ * value 1.875), nu (>= 0): 5-bit exponent, 3-bit mantissa, both with gradual
+ * underflow to 0; F = 255 marks a block holding a value that is not finite,
+ * all of which reads as NaN. The step rounds up or down at random, with the
+ * probabilities that keep the mean, from 16 bits of a hash of (seed, c,
+ * index of the tensor, block, element) for each moment; nu' > 0 never becomes
+ * 0. The parameter's update uses the new moments before they are rounded.
+ */
+GS_API int gs_adamw_step(const GsAdamwTensor* tensors, int n_tensors, const GsAdamwConfig* config,
+                         const float* grad_scale, int32_t* state, gs_stream_t stream);
+
+/*
+ * Global norm of a gradient (optax.global_norm) and the factor that clips it
+ * (optax.clip_by_global_norm): over all elements of all tensors,
+ *   norm  = u sqrt(sum grad^2),  u = *unscale (1 if NULL), e.g. 1 / loss scale
+ *   scale = u * (norm < max_norm ? 1 : max_norm / norm)
+ * scale is NaN when the norm is not finite (in fp32). &out->scale is a
+ * grad_scale for gs_adamw_step, which then clips, or skips the step, without
+ * the host. The squares are summed in fp64 in a fixed order. max_norm > 0,
+ * INFINITY for no clip. out: device, zeroed by the caller once. Workspace
+ * (8-byte aligned): gs_grad_norm_workspace_bytes(n_tensors) bytes; calls that
+ * overlap on the GPU need their own workspace and out.
+ */
+typedef struct GsGradTensor {
+  const void* grad;
+  int64_t count;
+  int32_t type;
+  int32_t reserved;
+} GsGradTensor;
+
+typedef struct GsGradNorm {
+  float norm;
+  float scale;
+  uint32_t ticket; /* used internally, 0 between calls */
+  int32_t reserved;
+} GsGradNorm;
+
+GS_API int gs_grad_norm(const GsGradTensor* tensors, int n_tensors, float max_norm, const float* unscale,
+                        GsGradNorm* out, void* workspace, size_t workspace_bytes, gs_stream_t stream);
+GS_API size_t gs_grad_norm_workspace_bytes(int n_tensors);
+
+/*
+ * 8-bit moments to values (type GS_TYPE_F32 or GS_TYPE_BF16, both exact but
+ * for values below the type's smallest) and back (to nearest, halves up;
+ * values that came from codes are kept exactly). count elements in
+ * ceil(count / 128) blocks; mu, nu, mu_exp, nu_exp as in GsAdamwTensor.
+ */
+GS_API int gs_moments8_decode(const uint8_t* mu, const uint8_t* nu, const uint8_t* mu_exp, const uint8_t* nu_exp,
+                              int64_t count, int type, void* mu_out, void* nu_out, gs_stream_t stream);
+GS_API int gs_moments8_encode(const float* mu, const float* nu, int64_t count, uint8_t* mu_codes,
+                              uint8_t* nu_codes, uint8_t* mu_exp, uint8_t* nu_exp, gs_stream_t stream);
+
 /* ---- density control ------------------------------------------------ */
 
 /*

@@ -27,6 +27,7 @@ SOURCES = [
     "gs_sort.cu",
     "gs_raster.cu",
     "gs_train.cu",
+    "gs_adamw.cu",
     "gs_ssim.cu",
     "gs_loss.cu",
     "gs_density.cu",

@@ -3,6 +3,7 @@
 // Host side only: argument validation, the workspace layout and the launch
 // sequence of each entry point. No allocation, no synchronisation.
 #include <algorithm>
+#include <cmath>
 #include <cstring>
 
 #include "gs_kernels.cuh"
@@ -650,6 +651,91 @@ int gs_grad2d_magnitude(const float* grad_means, const float* means, const float
   if (n < 0 || width <= 0 || height <= 0) return GS_ERR_INVALID_ARGUMENT;
   if (n > 0 && (!grad_means || !means || !w2c || !grad2d)) return GS_ERR_INVALID_ARGUMENT;
   launch_grad2d(grad_means, means, w2c, n, fx, fy, width, height, grad2d, stream);
+  return last_error();
+}
+
+// Elements of one tensor of gs_adamw_step / gs_grad_norm, and tiles of all
+// tensors of a call (the kernels index tiles in int32).
+constexpr int64_t kAdamwMaxCount = 1ll << 37;
+constexpr int64_t kAdamwMaxTiles = 1ll << 30;
+
+static bool misaligned(const void* p, size_t to) { return (((uintptr_t)p) & (to - 1)) != 0; }
+static size_t type_bytes(int type) { return type == GS_TYPE_F32 ? 4 : 2; }
+
+static int check_adamw_tensor(const GsAdamwTensor& t, int bits) {
+  if (t.count < 0 || t.count > kAdamwMaxCount) return GS_ERR_INVALID_ARGUMENT;
+  if (!std::isfinite(t.lr_init) || !std::isfinite(t.weight_decay)) return GS_ERR_INVALID_ARGUMENT;
+  if (!(t.decay_rate > 0.f) || !std::isfinite(t.decay_rate)) return GS_ERR_INVALID_ARGUMENT;
+  if (!(t.transition_steps > 0.f) || !std::isfinite(t.transition_steps)) return GS_ERR_INVALID_ARGUMENT;
+  if (t.grad_type < GS_TYPE_F32 || t.grad_type > GS_TYPE_F16) return GS_ERR_INVALID_ARGUMENT;
+  if (t.copy && t.copy_type != GS_TYPE_BF16 && t.copy_type != GS_TYPE_F16) return GS_ERR_INVALID_ARGUMENT;
+  if (t.active && (t.width < 1 || t.width > 65535 || t.count % t.width != 0)) return GS_ERR_INVALID_ARGUMENT;
+  if (t.count == 0) return GS_OK;
+  if (!t.param || !t.grad || !t.mu || !t.nu) return GS_ERR_INVALID_ARGUMENT;
+  if (misaligned(t.param, 4) || misaligned(t.grad, type_bytes(t.grad_type)) || misaligned(t.copy, 2))
+    return GS_ERR_INVALID_ARGUMENT;
+  if (misaligned(t.mu, 4) || misaligned(t.nu, 4)) return GS_ERR_INVALID_ARGUMENT;
+  if (bits == 8 && (!t.mu_exp || !t.nu_exp)) return GS_ERR_INVALID_ARGUMENT;
+  return GS_OK;
+}
+
+int gs_adamw_step(const GsAdamwTensor* tensors, int n_tensors, const GsAdamwConfig* config, const float* grad_scale,
+                  int32_t* state, gs_stream_t stream) {
+  if (n_tensors < 0 || (n_tensors > 0 && !tensors) || !config || !state) return GS_ERR_INVALID_ARGUMENT;
+  if (config->moment_bits != 32 && config->moment_bits != 8) return GS_ERR_INVALID_ARGUMENT;
+  if (!(config->b1 >= 0.0 && (float)config->b1 < 1.f) || !(config->b2 >= 0.0 && (float)config->b2 < 1.f))
+    return GS_ERR_INVALID_ARGUMENT;
+  if (!((float)config->eps > 0.f) || !std::isfinite((float)config->eps)) return GS_ERR_INVALID_ARGUMENT;
+  int64_t tiles = 0;
+  for (int i = 0; i < n_tensors; ++i) {
+    if (int s = check_adamw_tensor(tensors[i], config->moment_bits)) return s;
+    tiles += tensors[i].count / 1024 + 1;
+    if (tiles > kAdamwMaxTiles) return GS_ERR_TOO_LARGE;
+  }
+  launch_adamw(tensors, n_tensors, *config, grad_scale, state, (cudaStream_t)stream);
+  return last_error();
+}
+
+size_t gs_grad_norm_workspace_bytes(int n_tensors) { return n_tensors < 0 ? 0 : grad_norm_workspace_bytes(n_tensors); }
+
+int gs_grad_norm(const GsGradTensor* tensors, int n_tensors, float max_norm, const float* unscale, GsGradNorm* out,
+                 void* workspace, size_t workspace_bytes, gs_stream_t stream) {
+  if (n_tensors < 0 || (n_tensors > 0 && !tensors) || !out || !(max_norm > 0.f)) return GS_ERR_INVALID_ARGUMENT;
+  int64_t tiles = 0;
+  for (int i = 0; i < n_tensors; ++i) {
+    const GsGradTensor& t = tensors[i];
+    if (t.count < 0 || t.count > kAdamwMaxCount) return GS_ERR_INVALID_ARGUMENT;
+    if (t.type < GS_TYPE_F32 || t.type > GS_TYPE_F16) return GS_ERR_INVALID_ARGUMENT;
+    if (t.count > 0 && (!t.grad || misaligned(t.grad, type_bytes(t.type)))) return GS_ERR_INVALID_ARGUMENT;
+    tiles += t.count / 1024 + 1;
+    if (tiles > kAdamwMaxTiles) return GS_ERR_TOO_LARGE;
+  }
+  if (!workspace || workspace_bytes < grad_norm_workspace_bytes(n_tensors)) return GS_ERR_WORKSPACE_TOO_SMALL;
+  if (misaligned(workspace, 8)) return GS_ERR_INVALID_ARGUMENT;
+  launch_grad_norm(tensors, n_tensors, max_norm, unscale, out, workspace, (cudaStream_t)stream);
+  return last_error();
+}
+
+int gs_moments8_decode(const uint8_t* mu, const uint8_t* nu, const uint8_t* mu_exp, const uint8_t* nu_exp,
+                       int64_t count, int type, void* mu_out, void* nu_out, gs_stream_t stream) {
+  if (count < 0 || count > kAdamwMaxCount || (type != GS_TYPE_F32 && type != GS_TYPE_BF16))
+    return GS_ERR_INVALID_ARGUMENT;
+  if (count > 0 && (!mu || !nu || !mu_exp || !nu_exp || !mu_out || !nu_out)) return GS_ERR_INVALID_ARGUMENT;
+  if (misaligned(mu, 4) || misaligned(nu, 4)) return GS_ERR_INVALID_ARGUMENT;
+  if (misaligned(mu_out, type_bytes(type)) || misaligned(nu_out, type_bytes(type))) return GS_ERR_INVALID_ARGUMENT;
+  if (count == 0) return GS_OK;
+  launch_moments8_decode(mu, nu, mu_exp, nu_exp, count, type, mu_out, nu_out, (cudaStream_t)stream);
+  return last_error();
+}
+
+int gs_moments8_encode(const float* mu, const float* nu, int64_t count, uint8_t* mu_codes, uint8_t* nu_codes,
+                       uint8_t* mu_exp, uint8_t* nu_exp, gs_stream_t stream) {
+  if (count < 0 || count > kAdamwMaxCount) return GS_ERR_INVALID_ARGUMENT;
+  if (count > 0 && (!mu || !nu || !mu_codes || !nu_codes || !mu_exp || !nu_exp)) return GS_ERR_INVALID_ARGUMENT;
+  if (misaligned(mu, 4) || misaligned(nu, 4) || misaligned(mu_codes, 4) || misaligned(nu_codes, 4))
+    return GS_ERR_INVALID_ARGUMENT;
+  if (count == 0) return GS_OK;
+  launch_moments8_encode(mu, nu, count, mu_codes, nu_codes, mu_exp, nu_exp, (cudaStream_t)stream);
   return last_error();
 }
 

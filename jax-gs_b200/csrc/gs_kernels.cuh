@@ -256,6 +256,17 @@ void launch_density_stats(const float* grad2d, const float* radii, const uint8_t
                           const uint8_t* radii_valid, const uint8_t* active, int n,
                           float* grad_accum, int32_t* denom, float* max_radii, cudaStream_t st);
 
+// gs_adamw.cu: AdamW over many tensors, the gradient norm, 8-bit moments
+void launch_adamw(const GsAdamwTensor* tensors, int n, const GsAdamwConfig& cfg, const float* scale, int* state,
+                  cudaStream_t st);
+size_t grad_norm_workspace_bytes(int n);
+void launch_grad_norm(const GsGradTensor* tensors, int n, float max_norm, const float* unscale, GsGradNorm* out,
+                      void* ws, cudaStream_t st);
+void launch_moments8_decode(const uint8_t* mu, const uint8_t* nu, const uint8_t* mu_exp, const uint8_t* nu_exp,
+                            long long count, int type, void* mu_out, void* nu_out, cudaStream_t st);
+void launch_moments8_encode(const float* mu, const float* nu, long long count, uint8_t* mu8, uint8_t* nu8,
+                            uint8_t* mu_exp, uint8_t* nu_exp, cudaStream_t st);
+
 // gs_ssim.cu
 size_t dssim_workspace_bytes(int h, int w, int c);
 // Zero the ticket block of a D-SSIM workspace (before every launch_dssim).

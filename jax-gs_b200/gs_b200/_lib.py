@@ -49,6 +49,32 @@ class GsPeerSet(ctypes.Structure):
          "extras")]
 
 
+# Value types and the block of 8-bit moments (include/gsb200.h).
+GS_TYPE_F32, GS_TYPE_BF16, GS_TYPE_F16 = 0, 1, 2
+GS_ADAMW_BLOCK = 128
+
+
+class GsAdamwTensor(ctypes.Structure):
+    """struct GsAdamwTensor (include/gsb200.h)."""
+    _fields_ = [(name, ctypes.c_void_p) for name in
+                ("param", "grad", "mu", "nu", "mu_exp", "nu_exp", "copy", "active")] + [
+        ("count", ctypes.c_int64), ("width", ctypes.c_int32), ("grad_type", ctypes.c_int32),
+        ("copy_type", ctypes.c_int32), ("lr_init", ctypes.c_float), ("decay_rate", ctypes.c_float),
+        ("transition_steps", ctypes.c_float), ("weight_decay", ctypes.c_float), ("reserved", ctypes.c_int32)]
+
+
+class GsAdamwConfig(ctypes.Structure):
+    """struct GsAdamwConfig (include/gsb200.h)."""
+    _fields_ = [("b1", ctypes.c_double), ("b2", ctypes.c_double), ("eps", ctypes.c_double),
+                ("moment_bits", ctypes.c_int32), ("seed", ctypes.c_uint32)]
+
+
+class GsGradTensor(ctypes.Structure):
+    """struct GsGradTensor (include/gsb200.h)."""
+    _fields_ = [("grad", ctypes.c_void_p), ("count", ctypes.c_int64), ("type", ctypes.c_int32),
+                ("reserved", ctypes.c_int32)]
+
+
 SIGNATURES = {
     "gs_status_string": (ctypes.c_char_p, [_I]),
     "gs_version": (_I, []),
@@ -105,6 +131,11 @@ SIGNATURES = {
     "gs_grad2d_magnitude": (_I, [_P, _P, _P, _I, _F, _F, _I, _I, _P, _P]),
     "gs_accumulate_density_stats": (_I, [_P, _P, _P, _P, _P, _I, _P, _P, _P, _P]),
     "gs_density_step_stats": (_I, [_P, _P, _P, _I, _F, _F, _I, _I, _P, _P, _P, _P, _P, _P, _P, _P]),
+    "gs_adamw_step": (_I, [ctypes.POINTER(GsAdamwTensor), _I, ctypes.POINTER(GsAdamwConfig), _P, _P, _P]),
+    "gs_grad_norm": (_I, [ctypes.POINTER(GsGradTensor), _I, _F, _P, _P, _P, _S, _P]),
+    "gs_grad_norm_workspace_bytes": (_S, [_I]),
+    "gs_moments8_decode": (_I, [_P, _P, _P, _P, _L, _I, _P, _P, _P]),
+    "gs_moments8_encode": (_I, [_P, _P, _L, _P, _P, _P, _P, _P]),
     "gs_timing_enable": (_I, [_I]),
     "gs_timing_disable": (_I, []),
     "gs_timing_reset": (_I, []),
