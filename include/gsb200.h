@@ -559,7 +559,7 @@ typedef struct GsAdamwTensor {
   const uint8_t* active; /* nullable: count / width flags, flag r for elements
                             [r width, (r + 1) width) */
   int64_t count;         /* >= 0, at most 2^37 */
-  int32_t width;         /* 1 .. 65535; read where active is set */
+  int32_t width;         /* 1 .. 32768; read where active is set */
   int32_t grad_type;
   int32_t copy_type;     /* read where copy is set */
   float lr_init, decay_rate, transition_steps, weight_decay;

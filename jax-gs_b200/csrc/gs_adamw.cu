@@ -42,7 +42,12 @@ namespace gs {
 
 constexpr int kAdamwBlock = GS_ADAMW_BLOCK;  // elements of a quantisation block and of a warp's unit of work
 constexpr int kAdamwWarps = 8;
-constexpr int kAdamwTile = kAdamwBlock * kAdamwWarps;  // elements a CTA takes at a time
+#ifndef GS_ADAMW_UNROLL
+#define GS_ADAMW_UNROLL 2
+#endif
+constexpr int kAdamwUnroll = GS_ADAMW_UNROLL;  // blocks a warp has in flight
+constexpr int kAdamwChunk = kAdamwBlock * kAdamwUnroll;
+constexpr int kAdamwTile = kAdamwChunk * kAdamwWarps;  // elements a CTA takes at a time
 static_assert(kAdamwBlock == 128, "a warp holds a block, four elements a lane");
 
 // One tensor as the kernels see it.
@@ -58,7 +63,8 @@ struct AdamwDesc {
   long long count;
   float lr_init, ln_decay, weight_decay;  // lr = lr_init exp(c ln_decay)
   unsigned width;                         // elements per active flag
-  uint8_t grad_type, copy_type, pad[2];
+  unsigned long long magic;               // ceil(2^64 / width)
+  uint8_t grad_type, copy_type, vec, pad[5];
 };
 
 // Tables travel as kernel parameters (no device copy, nothing to keep alive,
@@ -130,8 +136,203 @@ struct AdamwStep {
 };
 
 __device__ __forceinline__ float adamw_param(float p, float m, float v, const AdamwStep& h, float eps) {
-  const float d = sqrtf(v * h.inv2) + eps;
+  float root;
+  asm("sqrt.approx.f32 %0, %1;" : "=f"(root) : "f"(v * h.inv2));
+  const float d = root + eps;
   return p - h.lr * (__fdividef(m * h.inv1, d) + h.wd * p);
+}
+
+// Element q of a lane in a block: four consecutive elements a lane (16-byte
+// accesses), or, where a pointer is not aligned for that, every 32nd.
+template <bool VEC>
+__device__ __forceinline__ int block_element(int lane, int q) {
+  return VEC ? 4 * lane + q : lane + 32 * q;
+}
+
+template <bool VEC>
+__device__ __forceinline__ void load4(const float* __restrict__ p, int lane, float x[4]) {
+  if (VEC) {
+    const float4 t = reinterpret_cast<const float4*>(p)[lane];
+    x[0] = t.x; x[1] = t.y; x[2] = t.z; x[3] = t.w;
+  } else {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) x[q] = p[lane + 32 * q];
+  }
+}
+
+template <bool VEC>
+__device__ __forceinline__ void store4(float* __restrict__ p, int lane, const float x[4]) {
+  if (VEC) {
+    reinterpret_cast<float4*>(p)[lane] = make_float4(x[0], x[1], x[2], x[3]);
+  } else {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) p[lane + 32 * q] = x[q];
+  }
+}
+
+// Four gradients as loaded (16-bit ones two to a register where VEC).
+template <int GT, bool VEC>
+struct Grad4 {
+  uint32_t w[(GT == GS_TYPE_F32 || !VEC) ? 4 : 2];
+  __device__ __forceinline__ void load(const void* g, long long base, int lane) {
+    if (GT == GS_TYPE_F32) {
+      float x[4];
+      load4<VEC>(static_cast<const float*>(g) + base, lane, x);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) w[q] = __float_as_uint(x[q]);
+    } else if (VEC) {
+      const uint2 t = reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(g) + base)[lane];
+      w[0] = t.x;
+      w[1] = t.y;
+    } else {
+#pragma unroll
+      for (int q = 0; q < 4; ++q) w[q] = (static_cast<const uint16_t*>(g) + base)[lane + 32 * q];
+    }
+  }
+  __device__ __forceinline__ float get(int q) const {
+    if (GT == GS_TYPE_F32) return __uint_as_float(w[q]);
+    const unsigned h = VEC ? (q & 1 ? w[q >> 1] >> 16 : w[q >> 1] & 0xFFFFu) : w[q];
+    if (GT == GS_TYPE_BF16) return __uint_as_float(h << 16);
+    return __half2float(__ushort_as_half((unsigned short)h));
+  }
+};
+
+template <bool VEC>
+__device__ __forceinline__ void store_copy4(void* p, long long base, int lane, int type, const float x[4]) {
+  unsigned h[4];
+#pragma unroll
+  for (int q = 0; q < 4; ++q)
+    h[q] = type == GS_TYPE_BF16 ? __bfloat16_as_ushort(__float2bfloat16_rn(x[q]))
+                                : __half_as_ushort(__float2half_rn(x[q]));
+  uint16_t* c = static_cast<uint16_t*>(p) + base;
+  if (VEC) {
+    reinterpret_cast<uint2*>(c)[lane] = make_uint2(h[0] | (h[1] << 16), h[2] | (h[3] << 16));
+  } else {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) c[lane + 32 * q] = (uint16_t)h[q];
+  }
+}
+
+// Four codes, one to a byte.
+template <bool VEC>
+__device__ __forceinline__ unsigned load_codes(const void* p, long long base, int lane) {
+  const uint8_t* c = static_cast<const uint8_t*>(p) + base;
+  if (VEC) return reinterpret_cast<const unsigned*>(c)[lane];
+  unsigned w = 0u;
+#pragma unroll
+  for (int q = 0; q < 4; ++q) w |= (unsigned)c[lane + 32 * q] << (8 * q);
+  return w;
+}
+
+template <bool VEC>
+__device__ __forceinline__ void store_codes(void* p, long long base, int lane, unsigned w) {
+  uint8_t* c = static_cast<uint8_t*>(p) + base;
+  if (VEC) {
+    reinterpret_cast<unsigned*>(c)[lane] = w;
+  } else {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) c[lane + 32 * q] = (uint8_t)(w >> (8 * q));
+  }
+}
+
+// Whole blocks of a tensor by one warp, all loads issued before the first use.
+template <int BITS, int GT, bool VEC>
+__device__ __forceinline__ void adamw_chunk(const AdamwDesc& d, long long base, const AdamwParams& a,
+                                            const AdamwStep& h, float s, unsigned key) {
+  constexpr int U = kAdamwUnroll;
+  const int lane = threadIdx.x & 31;
+  float p[U][4], m[U][4], v[U][4];
+  Grad4<GT, VEC> g[U];
+  unsigned cm[U], cv[U];
+  int fm[U], fv[U];
+  const long long blk0 = base / kAdamwBlock;
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const long long b = base + u * kAdamwBlock;
+    load4<VEC>(d.param + b, lane, p[u]);
+    g[u].load(d.grad, b, lane);
+    if (BITS == 8) {
+      cm[u] = load_codes<VEC>(d.mu, b, lane);
+      cv[u] = load_codes<VEC>(d.nu, b, lane);
+      fm[u] = d.mu_exp[blk0 + u];
+      fv[u] = d.nu_exp[blk0 + u];
+    } else {
+      load4<VEC>(static_cast<const float*>(d.mu) + b, lane, m[u]);
+      load4<VEC>(static_cast<const float*>(d.nu) + b, lane, v[u]);
+    }
+  }
+  unsigned act = 0xFFFFFFFFu;
+  if (d.active) {
+    // row of element e: (base + e) / width, by multiplications with the
+    // rounded-up reciprocal (exact: base < 2^37 and width <= 2^15, so that
+    // their product with the reciprocal's excess stays below its scale)
+    const unsigned w = d.width;
+    const unsigned long long row0 = w == 1 ? (unsigned long long)base : __umul64hi((unsigned long long)base, d.magic);
+    const unsigned rem0 = (unsigned)((unsigned long long)base - row0 * w);
+    const unsigned magic = (unsigned)(d.magic >> 32) + 1u;  // > 2^32 / width
+    const uint8_t* flags = d.active + row0;
+    act = 0u;
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const unsigned x = rem0 + u * kAdamwBlock + block_element<VEC>(lane, q);
+        const unsigned r = w == 1 ? x : __umulhi(x, magic);
+        act |= (flags[r] != 0 ? 1u : 0u) << (4 * u + q);
+      }
+  }
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const long long b = base + u * kAdamwBlock;
+    float up_m = 0.f, up_v = 0.f;
+    if (BITS == 8) {
+      up_m = pow2_biased(min(fm[u], 254));
+      up_v = pow2_biased(min(fv[u], 254));
+      if (fm[u] == 255) up_m = NAN;
+      if (fv[u] == 255) up_v = NAN;
+    }
+    unsigned top_m = 0u, top_v = 0u;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      if (BITS == 8) {
+        m[u][q] = decode8<true>((cm[u] >> (8 * q)) & 255u, up_m);
+        v[u][q] = decode8<false>((cv[u] >> (8 * q)) & 255u, up_v);
+      }
+      const float gq = g[u].get(q) * s;
+      m[u][q] = add_rn(mul_rn(m[u][q], a.b1), mul_rn(gq, a.omb1));
+      v[u][q] = add_rn(mul_rn(v[u][q], a.b2), mul_rn(mul_rn(gq, gq), a.omb2));
+      const float fresh = adamw_param(p[u][q], m[u][q], v[u][q], h, a.eps);
+      if ((act >> (4 * u + q)) & 1u) p[u][q] = fresh;
+      if (BITS == 8) {
+        top_m = max(top_m, __float_as_uint(fabsf(m[u][q])));
+        top_v = max(top_v, __float_as_uint(v[u][q]) & 0x7FFFFFFFu);
+      }
+    }
+    store4<VEC>(d.param + b, lane, p[u]);
+    if (d.copy) store_copy4<VEC>(d.copy, b, lane, d.copy_type, p[u]);
+    if (BITS == 32) {
+      store4<VEC>(static_cast<float*>(d.mu) + b, lane, m[u]);
+      store4<VEC>(static_cast<float*>(d.nu) + b, lane, v[u]);
+    } else {
+      const int nm = block_field(__reduce_max_sync(0xffffffffu, top_m));
+      const int nv = block_field(__reduce_max_sync(0xffffffffu, top_v));
+      const float down_m = pow2_biased(max(254 - nm, 0)), down_v = pow2_biased(max(254 - nv, 0));
+      const unsigned bkey = mix32(key ^ (unsigned)(blk0 + u));
+      unsigned wm = 0u, wv = 0u;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const unsigned r = mix32(bkey + kGolden * (unsigned)block_element<VEC>(lane, q));
+        wm |= encode8<true>(m[u][q], down_m, (r & 0xFFFFu) << 4) << (8 * q);
+        wv |= encode8<false>(v[u][q], down_v, (r >> 16) << 4) << (8 * q);
+      }
+      store_codes<VEC>(d.mu, b, lane, nm == 255 ? 0u : wm);
+      store_codes<VEC>(d.nu, b, lane, nv == 255 ? 0u : wv);
+      if (lane == 0) {
+        d.mu_exp[blk0 + u] = (uint8_t)nm;
+        d.nu_exp[blk0 + u] = (uint8_t)nv;
+      }
+    }
+  }
 }
 
 // One block of a tensor by one warp, `rem` elements of it in range.
@@ -234,11 +435,23 @@ k_adamw(const __grid_constant__ AdamwTable<N> tab, const __grid_constant__ Adamw
       const AdamwDesc& d = tab.t[k];
       h.lr = d.lr_init * expf(cf * d.ln_decay);
       h.wd = d.weight_decay;
-      const long long base = (long long)(tile - tab.first[k]) * kAdamwTile + (threadIdx.x >> 5) * kAdamwBlock;
+      const long long base = (long long)(tile - tab.first[k]) * kAdamwTile + (threadIdx.x >> 5) * kAdamwChunk;
       const long long left = d.count - base;
       if (left <= 0) continue;
       const unsigned tkey = mix32(key + kGolden * (unsigned)(tab.index0 + k));
-      adamw_block<BITS>(d, base, (int)(left < kAdamwBlock ? left : kAdamwBlock), a, h, s, tkey);
+      if (left >= kAdamwChunk) {
+        switch (d.grad_type * 2 + d.vec) {
+          case 0: adamw_chunk<BITS, GS_TYPE_F32, false>(d, base, a, h, s, tkey); break;
+          case 1: adamw_chunk<BITS, GS_TYPE_F32, true>(d, base, a, h, s, tkey); break;
+          case 2: adamw_chunk<BITS, GS_TYPE_BF16, false>(d, base, a, h, s, tkey); break;
+          case 3: adamw_chunk<BITS, GS_TYPE_BF16, true>(d, base, a, h, s, tkey); break;
+          case 4: adamw_chunk<BITS, GS_TYPE_F16, false>(d, base, a, h, s, tkey); break;
+          default: adamw_chunk<BITS, GS_TYPE_F16, true>(d, base, a, h, s, tkey); break;
+        }
+      } else {
+        for (int e = 0; e < left; e += kAdamwBlock)
+          adamw_block<BITS>(d, base + e, (int)(left - e < kAdamwBlock ? left - e : kAdamwBlock), a, h, s, tkey);
+      }
     }
   }
   if (!a.advance) return;
@@ -276,6 +489,11 @@ static void launch_adamw_class(const GsAdamwTensor* t, int n, int index0, const 
     d.width = (unsigned)t[i].width;
     d.grad_type = (uint8_t)t[i].grad_type;
     d.copy_type = (uint8_t)t[i].copy_type;
+    d.magic = t[i].width > 1 ? ~0ull / (unsigned)t[i].width + 1ull : 0ull;
+    const size_t g4 = t[i].grad_type == GS_TYPE_F32 ? 16 : 8;
+    uintptr_t bits = (uintptr_t)t[i].param | ((uintptr_t)t[i].copy * 2) | ((uintptr_t)t[i].grad * (16 / g4));
+    if (BITS == 32) bits |= (uintptr_t)t[i].mu | (uintptr_t)t[i].nu;
+    d.vec = (bits & 15) == 0;
     tab.first[i] = tiles;
     tiles += (int)((t[i].count + kAdamwTile - 1) / kAdamwTile);
   }
@@ -336,7 +554,62 @@ struct GradTable {
   int n;
 };
 
-constexpr int kNormTile = 2048;
+// A tile is 16 KB of a tensor counted from the 16-byte boundary at or before
+// its first element, 64 bytes a thread in 16-byte loads; only the vectors
+// that hold both the tensor's elements and others are read one by one.
+constexpr int kNormVecs = 4;
+constexpr int kNormTileBytes = 256 * 16 * kNormVecs;
+
+__host__ __device__ __forceinline__ long long norm_tiles(const void* grad, long long count, int type) {
+  const long long bytes = (long long)((uintptr_t)grad & 15) + count * (type == GS_TYPE_F32 ? 4 : 2);
+  return count > 0 ? (bytes + kNormTileBytes - 1) / kNormTileBytes : 0;
+}
+
+template <int GT>
+__device__ __forceinline__ void norm_tile(const GradDesc& d, long long tile, double acc[4]) {
+  constexpr int PER = GT == GS_TYPE_F32 ? 4 : 8;  // elements of a vector
+  const unsigned shift = (unsigned)((uintptr_t)d.grad & 15) / (16 / PER);
+  const uint4* vecs = reinterpret_cast<const uint4*>((uintptr_t)d.grad & ~(uintptr_t)15);
+  const long long v0 = tile * (256 * kNormVecs) + threadIdx.x;
+  uint4 w[kNormVecs];
+#pragma unroll
+  for (int j = 0; j < kNormVecs; ++j) {
+    const long long e = (v0 + 256 * j) * PER - shift;  // the vector's first element
+    w[j] = make_uint4(0u, 0u, 0u, 0u);
+    if (e >= 0 && e + PER <= d.count) {
+      w[j] = __ldg(vecs + v0 + 256 * j);
+    } else if (e + PER > 0 && e < d.count) {
+      for (int q = 0; q < PER; ++q)
+        if (e + q >= 0 && e + q < d.count) {
+          const double x = (double)load_as_float(d.grad, e + q, GT);
+          acc[0] += x * x;
+        }
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < kNormVecs; ++j) {
+    const unsigned b[4] = {w[j].x, w[j].y, w[j].z, w[j].w};
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      if (GT == GS_TYPE_F32) {
+        const double x = (double)__uint_as_float(b[q]);
+        acc[q] = fma(x, x, acc[q]);
+      } else {
+        float lo, hi;
+        if (GT == GS_TYPE_BF16) {
+          lo = __uint_as_float(b[q] << 16);
+          hi = __uint_as_float(b[q] & 0xFFFF0000u);
+        } else {
+          lo = __half2float(__ushort_as_half((unsigned short)(b[q] & 0xFFFFu)));
+          hi = __half2float(__ushort_as_half((unsigned short)(b[q] >> 16)));
+        }
+        const double x = (double)lo, y = (double)hi;
+        acc[q] = fma(x, x, acc[q]);
+        acc[q] = fma(y, y, acc[q]);
+      }
+    }
+  }
+}
 
 template <int N>
 __global__ void __launch_bounds__(256)
@@ -345,7 +618,7 @@ k_grad_norm(const __grid_constant__ GradTable<N> tab, double* __restrict__ parti
   GS_PDL_ENTRY_PLAIN();
   __shared__ double s_red[8];
   __shared__ bool s_last;
-  double acc = 0.0;
+  double sums[4] = {0.0, 0.0, 0.0, 0.0};
   const int tiles = tab.first[tab.n];
   int k = 0;
   for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
@@ -356,12 +629,12 @@ k_grad_norm(const __grid_constant__ GradTable<N> tab, double* __restrict__ parti
       else hi = mid;
     }
     const GradDesc& d = tab.t[k];
-    const long long base = (long long)(tile - tab.first[k]) * kNormTile;
-    for (int e = threadIdx.x; e < kNormTile && base + e < d.count; e += 256) {
-      const double g = (double)load_as_float(d.grad, base + e, d.type);
-      acc += g * g;
-    }
+    const long long t = tile - tab.first[k];
+    if (d.type == GS_TYPE_F32) norm_tile<GS_TYPE_F32>(d, t, sums);
+    else if (d.type == GS_TYPE_BF16) norm_tile<GS_TYPE_BF16>(d, t, sums);
+    else norm_tile<GS_TYPE_F16>(d, t, sums);
   }
+  double acc = (sums[0] + sums[1]) + (sums[2] + sums[3]);
   acc = block_sum_d256(acc, s_red);
   if (threadIdx.x == 0) {
     partials[part0 + blockIdx.x] = acc;
@@ -396,7 +669,7 @@ static int fill_grad_table(const GsGradTensor* t, int n, GradTable<N>& tab) {
     tab.t[i].count = t[i].count;
     tab.t[i].type = t[i].type;
     tab.first[i] = tiles;
-    tiles += (int)((t[i].count + kNormTile - 1) / kNormTile);
+    tiles += (int)norm_tiles(t[i].grad, t[i].count, t[i].type);
   }
   tab.first[n] = tiles;
   tab.n = n;
@@ -412,7 +685,7 @@ size_t grad_norm_workspace_bytes(int n) {
 
 static int norm_grid(const GsGradTensor* t, int n) {
   long long tiles = 0;
-  for (int i = 0; i < n; ++i) tiles += (t[i].count + kNormTile - 1) / kNormTile;
+  for (int i = 0; i < n; ++i) tiles += norm_tiles(t[i].grad, t[i].count, t[i].type);
   return (int)std::max(1ll, std::min(tiles, (long long)kNormGrid));
 }
 

@@ -669,7 +669,7 @@ static int check_adamw_tensor(const GsAdamwTensor& t, int bits) {
   if (!(t.transition_steps > 0.f) || !std::isfinite(t.transition_steps)) return GS_ERR_INVALID_ARGUMENT;
   if (t.grad_type < GS_TYPE_F32 || t.grad_type > GS_TYPE_F16) return GS_ERR_INVALID_ARGUMENT;
   if (t.copy && t.copy_type != GS_TYPE_BF16 && t.copy_type != GS_TYPE_F16) return GS_ERR_INVALID_ARGUMENT;
-  if (t.active && (t.width < 1 || t.width > 65535 || t.count % t.width != 0)) return GS_ERR_INVALID_ARGUMENT;
+  if (t.active && (t.width < 1 || t.width > 32768 || t.count % t.width != 0)) return GS_ERR_INVALID_ARGUMENT;
   if (t.count == 0) return GS_OK;
   if (!t.param || !t.grad || !t.mu || !t.nu) return GS_ERR_INVALID_ARGUMENT;
   if (misaligned(t.param, 4) || misaligned(t.grad, type_bytes(t.grad_type)) || misaligned(t.copy, 2))

@@ -315,8 +315,8 @@ class AdamW(_Plan):
                 rows = t.param.shape[0] if t.param.dim() else 1
                 if t.active.numel() != rows:
                     raise ValueError(f"{name}.active: {t.active.numel()} flags, expected {rows}")
-                if rows and n // rows > 65535:
-                    raise ValueError(f"{name}.active: rows of {n // rows} elements, at most 65535")
+                if rows and n // rows > 32768:
+                    raise ValueError(f"{name}.active: rows of {n // rows} elements, at most 32768")
                 read.append((f"{name}.active", t.active))
             if self.moment_bits == 32:
                 for key, m in zip(("mu", "nu"), self.moments[i]):

@@ -38,7 +38,7 @@ BAD_TENSORS = [
     dict(count=-1), dict(count=(1 << 37) + 1), dict(param=None), dict(grad=None), dict(mu=None), dict(nu=None),
     dict(param=P + 2), dict(mu=P + 1), dict(nu=P + 2), dict(grad=P + 2), dict(grad=P + 1, grad_type=1),
     dict(grad_type=3), dict(grad_type=-1), dict(copy=P, copy_type=0), dict(copy=P, copy_type=3),
-    dict(copy=P + 1, copy_type=1), dict(active=P, width=0), dict(active=P, width=3), dict(active=P, width=65536),
+    dict(copy=P + 1, copy_type=1), dict(active=P, width=0), dict(active=P, width=3), dict(active=P, width=32769, count=32769),
     dict(lr_init=math.nan), dict(lr_init=math.inf), dict(weight_decay=math.nan), dict(decay_rate=0.0),
     dict(decay_rate=math.inf), dict(transition_steps=0.0), dict(transition_steps=math.nan),
 ]
