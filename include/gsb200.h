@@ -568,7 +568,7 @@ typedef struct GsAdamwTensor {
 
 typedef struct GsAdamwConfig {
   double b1, b2;        /* in [0, 1) */
-  double eps;           /* > 0, also as a float */
+  double eps;           /* > 0, a normal number as a float */
   int32_t moment_bits;  /* 32 or 8 */
   uint32_t seed;        /* moment_bits 8: of the stochastic rounding */
 } GsAdamwConfig;

@@ -42,13 +42,16 @@ namespace gs {
 
 constexpr int kAdamwBlock = GS_ADAMW_BLOCK;  // elements of a quantisation block and of a warp's unit of work
 constexpr int kAdamwWarps = 8;
-#ifndef GS_ADAMW_UNROLL
-#define GS_ADAMW_UNROLL 2
-#endif
-constexpr int kAdamwUnroll = GS_ADAMW_UNROLL;  // blocks a warp has in flight
+constexpr int kAdamwUnroll = 2;  // blocks of a chunk, what a warp takes at a time
 constexpr int kAdamwChunk = kAdamwBlock * kAdamwUnroll;
 constexpr int kAdamwTile = kAdamwChunk * kAdamwWarps;  // elements a CTA takes at a time
 static_assert(kAdamwBlock == 128, "a warp holds a block, four elements a lane");
+#ifndef GS_ADAMW_CTAS
+#define GS_ADAMW_CTAS 3
+#endif
+#ifndef GS_ADAMW8_CTAS
+#define GS_ADAMW8_CTAS 4
+#endif
 
 // One tensor as the kernels see it.
 struct AdamwDesc {
@@ -135,11 +138,20 @@ struct AdamwStep {
   float lr, wd, inv1, inv2;
 };
 
+// eps is a normal float, so the denominator is one and lies far below 2^126:
+// the reciprocal needs no care for subnormals (the square root does).
 __device__ __forceinline__ float adamw_param(float p, float m, float v, const AdamwStep& h, float eps) {
-  float root;
+  float root, inv;
   asm("sqrt.approx.f32 %0, %1;" : "=f"(root) : "f"(v * h.inv2));
-  const float d = root + eps;
-  return p - h.lr * (__fdividef(m * h.inv1, d) + h.wd * p);
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(root + eps));
+  return p - h.lr * ((m * h.inv1) * inv + h.wd * p);
+}
+
+// max(a, |b|), NaN if one is
+__device__ __forceinline__ float max_abs(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(fabsf(b)));
+  return r;
 }
 
 // Element q of a lane in a block: four consecutive elements a lane (16-byte
@@ -149,24 +161,26 @@ __device__ __forceinline__ int block_element(int lane, int q) {
   return VEC ? 4 * lane + q : lane + 32 * q;
 }
 
+// Accesses are a pointer that is the same in all threads plus a 32-bit
+// element offset `i` of the lane's first element.
 template <bool VEC>
-__device__ __forceinline__ void load4(const float* __restrict__ p, int lane, float x[4]) {
+__device__ __forceinline__ void load4(const float* p, unsigned i, float x[4]) {
   if (VEC) {
-    const float4 t = reinterpret_cast<const float4*>(p)[lane];
+    const float4 t = *reinterpret_cast<const float4*>(p + i);
     x[0] = t.x; x[1] = t.y; x[2] = t.z; x[3] = t.w;
   } else {
 #pragma unroll
-    for (int q = 0; q < 4; ++q) x[q] = p[lane + 32 * q];
+    for (int q = 0; q < 4; ++q) x[q] = p[i + 32 * q];
   }
 }
 
 template <bool VEC>
-__device__ __forceinline__ void store4(float* __restrict__ p, int lane, const float x[4]) {
+__device__ __forceinline__ void store4(float* p, unsigned i, const float x[4]) {
   if (VEC) {
-    reinterpret_cast<float4*>(p)[lane] = make_float4(x[0], x[1], x[2], x[3]);
+    *reinterpret_cast<float4*>(p + i) = make_float4(x[0], x[1], x[2], x[3]);
   } else {
 #pragma unroll
-    for (int q = 0; q < 4; ++q) p[lane + 32 * q] = x[q];
+    for (int q = 0; q < 4; ++q) p[i + 32 * q] = x[q];
   }
 }
 
@@ -174,19 +188,19 @@ __device__ __forceinline__ void store4(float* __restrict__ p, int lane, const fl
 template <int GT, bool VEC>
 struct Grad4 {
   uint32_t w[(GT == GS_TYPE_F32 || !VEC) ? 4 : 2];
-  __device__ __forceinline__ void load(const void* g, long long base, int lane) {
+  __device__ __forceinline__ void load(const void* g, unsigned i) {
     if (GT == GS_TYPE_F32) {
       float x[4];
-      load4<VEC>(static_cast<const float*>(g) + base, lane, x);
+      load4<VEC>(static_cast<const float*>(g), i, x);
 #pragma unroll
       for (int q = 0; q < 4; ++q) w[q] = __float_as_uint(x[q]);
     } else if (VEC) {
-      const uint2 t = reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(g) + base)[lane];
+      const uint2 t = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(g) + i);
       w[0] = t.x;
       w[1] = t.y;
     } else {
 #pragma unroll
-      for (int q = 0; q < 4; ++q) w[q] = (static_cast<const uint16_t*>(g) + base)[lane + 32 * q];
+      for (int q = 0; q < 4; ++q) w[q] = static_cast<const uint16_t*>(g)[i + 32 * q];
     }
   }
   __device__ __forceinline__ float get(int q) const {
@@ -198,264 +212,279 @@ struct Grad4 {
 };
 
 template <bool VEC>
-__device__ __forceinline__ void store_copy4(void* p, long long base, int lane, int type, const float x[4]) {
+__device__ __forceinline__ void store_copy4(void* p, unsigned i, int type, const float x[4]) {
   unsigned h[4];
 #pragma unroll
   for (int q = 0; q < 4; ++q)
     h[q] = type == GS_TYPE_BF16 ? __bfloat16_as_ushort(__float2bfloat16_rn(x[q]))
                                 : __half_as_ushort(__float2half_rn(x[q]));
-  uint16_t* c = static_cast<uint16_t*>(p) + base;
+  uint16_t* c = static_cast<uint16_t*>(p);
   if (VEC) {
-    reinterpret_cast<uint2*>(c)[lane] = make_uint2(h[0] | (h[1] << 16), h[2] | (h[3] << 16));
+    *reinterpret_cast<uint2*>(c + i) = make_uint2(h[0] | (h[1] << 16), h[2] | (h[3] << 16));
   } else {
 #pragma unroll
-    for (int q = 0; q < 4; ++q) c[lane + 32 * q] = (uint16_t)h[q];
+    for (int q = 0; q < 4; ++q) c[i + 32 * q] = (uint16_t)h[q];
   }
 }
 
 // Four codes, one to a byte.
 template <bool VEC>
-__device__ __forceinline__ unsigned load_codes(const void* p, long long base, int lane) {
-  const uint8_t* c = static_cast<const uint8_t*>(p) + base;
-  if (VEC) return reinterpret_cast<const unsigned*>(c)[lane];
+__device__ __forceinline__ unsigned load_codes(const uint8_t* c, unsigned i) {
+  if (VEC) return *reinterpret_cast<const unsigned*>(c + i);
   unsigned w = 0u;
 #pragma unroll
-  for (int q = 0; q < 4; ++q) w |= (unsigned)c[lane + 32 * q] << (8 * q);
+  for (int q = 0; q < 4; ++q) w |= (unsigned)c[i + 32 * q] << (8 * q);
   return w;
 }
 
 template <bool VEC>
-__device__ __forceinline__ void store_codes(void* p, long long base, int lane, unsigned w) {
-  uint8_t* c = static_cast<uint8_t*>(p) + base;
+__device__ __forceinline__ void store_codes(uint8_t* c, unsigned i, unsigned w) {
   if (VEC) {
-    reinterpret_cast<unsigned*>(c)[lane] = w;
+    *reinterpret_cast<unsigned*>(c + i) = w;
   } else {
 #pragma unroll
-    for (int q = 0; q < 4; ++q) c[lane + 32 * q] = (uint8_t)(w >> (8 * q));
+    for (int q = 0; q < 4; ++q) c[i + 32 * q] = (uint8_t)(w >> (8 * q));
   }
 }
 
-// Whole blocks of a tensor by one warp, all loads issued before the first use.
-template <int BITS, int GT, bool VEC>
-__device__ __forceinline__ void adamw_chunk(const AdamwDesc& d, long long base, const AdamwParams& a,
-                                            const AdamwStep& h, float s, unsigned key) {
+// Place of an element in the rows of an active mask: row and rest. Divisions
+// by the width are multiplications with its rounded-up reciprocal, exact
+// because the numerator times the reciprocal's excess (below the width, at
+// most 2^15) stays below the reciprocal's scale: elements < 2^37 under 2^64,
+// and a rest plus a chunk, below 2^16, under 2^32.
+struct RowPlace {
+  const uint8_t* flags;  // of the row
+  unsigned rest;
+
+  static __device__ __forceinline__ unsigned rows(const AdamwDesc& d, unsigned x) {
+    return d.width == 1 ? x : __umulhi(x, (unsigned)(d.magic >> 32) + 1u);
+  }
+  __device__ __forceinline__ void start(const AdamwDesc& d, unsigned long long e) {
+    const unsigned long long row = d.width == 1 ? e : __umul64hi(e, d.magic);
+    flags = d.active + row;
+    rest = (unsigned)(e - row * d.width);
+  }
+};
+
+// Flags of a lane's elements in U blocks that start `off` elements on, one bit each.
+template <bool VEC, int U>
+__device__ __forceinline__ unsigned active_bits(const AdamwDesc& d, const RowPlace& at, unsigned off, int lane) {
+  unsigned act = 0u;
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    if (VEC && d.width >= 4) {  // at most two rows in four elements
+      const unsigned x = at.rest + off + u * kAdamwBlock + 4 * lane;
+      const unsigned r = at.rows(d, x);
+      const unsigned left = (r + 1) * d.width - x;  // elements up to the next row
+      const unsigned head = left >= 4 ? 15u : (1u << left) - 1u;
+      unsigned bits = at.flags[r] != 0 ? head : 0u;
+      if (left < 4 && at.flags[r + 1] != 0) bits |= 15u & ~head;
+      act |= bits << (4 * u);
+    } else {
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const unsigned r = at.rows(d, at.rest + off + u * kAdamwBlock + block_element<VEC>(lane, q));
+        act |= (at.flags[r] != 0 ? 1u : 0u) << (4 * u + q);
+      }
+    }
+  }
+  return act;
+}
+
+// b times the four moments that a word of codes and an exponent byte stand
+// for. Where the value of every code is a normal float (F >= 18 or 34) and b
+// 2^(F - 127) 2^112 or 2^96 one too, b is folded into the scale: the same
+// single rounding of the same product.
+template <bool SIGNED>
+__device__ __forceinline__ void decayed4(unsigned w, int field, float b, float x[4]) {
+  constexpr int kLow = SIGNED ? 18 : 34, kShift = SIGNED ? 15 : 31;
+  if (field >= kLow && field <= 127 + kShift) {
+    const float k = __int_as_float((field - kShift + 127) << 23) * b;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      unsigned y;
+      if (SIGNED) y = (unsigned)((int)__byte_perm(w, 0u, 0x0444 | (q << 12)) >> 4) & 0x87F00000u;
+      else y = (q < 3 ? w << (20 - 8 * q) : w >> 4) & 0x0FF00000u;
+      x[q] = mul_rn(__uint_as_float(y), k);
+    }
+  } else {
+    const float up = field == 255 ? NAN : pow2_biased(field);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) x[q] = mul_rn(decode8<SIGNED>((w >> (8 * q)) & 255u, up), b);
+  }
+}
+
+// encode8 of four values under their block's exponent byte, one code a byte.
+// The scale is a single power of two while 2^(127 - F) 2^-112 or 2^-96 is a
+// normal float. No code exceeds the largest: F leaves the largest magnitude
+// at most at the top code, and noise is less than the next code away.
+template <bool SIGNED>
+__device__ __forceinline__ unsigned encode4(const float x[4], int field, const unsigned noise[4]) {
+  constexpr int kShift = SIGNED ? 15 : 31;
+  float scale, z[4] = {x[0], x[1], x[2], x[3]};
+  if (field <= 126 + kShift) {
+    scale = __int_as_float((127 + kShift - field) << 23);
+  } else {
+    const float first = pow2_biased(max(254 - field, 0));
+#pragma unroll
+    for (int q = 0; q < 4; ++q) z[q] *= first;
+    scale = SIGNED ? 0x1p-112f : 0x1p-96f;
+  }
+  unsigned c[4];
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    const float y = z[q] * scale;
+    if (SIGNED) {
+      const unsigned t = __float_as_uint(y) + noise[q];
+      c[q] = ((t << 4) & 0x7FFFFFFFu) | (t & 0x80000000u);
+    } else {
+      unsigned t = __float_as_uint(y) + noise[q];
+      if (x[q] > 0.f) t = max(t, 1u << 20);
+      c[q] = t << 4;
+    }
+  }
+  const unsigned w = __byte_perm(__byte_perm(c[0], c[1], 0x0073), __byte_perm(c[2], c[3], 0x0073), 0x5410);
+  return field == 255 ? 0u : w;
+}
+
+// Whole blocks with 32-bit moments from element `base` by one warp, all loads
+// issued before the first use.
+template <int GT, bool VEC>
+__device__ __forceinline__ void adamw32_chunk(const AdamwDesc& d, long long base, const AdamwParams& a,
+                                              const AdamwStep& h, float s) {
   constexpr int U = kAdamwUnroll;
   const int lane = threadIdx.x & 31;
   float p[U][4], m[U][4], v[U][4];
   Grad4<GT, VEC> g[U];
-  unsigned cm[U], cv[U];
-  int fm[U], fv[U];
-  const long long blk0 = base / kAdamwBlock;
+  float* const param = d.param + base;
+  float* const mu = static_cast<float*>(d.mu) + base;
+  float* const nu = static_cast<float*>(d.nu) + base;
+  const unsigned i0 = block_element<VEC>(lane, 0);
 #pragma unroll
   for (int u = 0; u < U; ++u) {
-    const long long b = base + u * kAdamwBlock;
-    load4<VEC>(d.param + b, lane, p[u]);
-    g[u].load(d.grad, b, lane);
-    if (BITS == 8) {
-      cm[u] = load_codes<VEC>(d.mu, b, lane);
-      cv[u] = load_codes<VEC>(d.nu, b, lane);
-      fm[u] = d.mu_exp[blk0 + u];
-      fv[u] = d.nu_exp[blk0 + u];
-    } else {
-      load4<VEC>(static_cast<const float*>(d.mu) + b, lane, m[u]);
-      load4<VEC>(static_cast<const float*>(d.nu) + b, lane, v[u]);
-    }
+    const unsigned i = i0 + u * kAdamwBlock;
+    load4<VEC>(param, i, p[u]);
+    g[u].load(static_cast<const char*>(d.grad) + base * (GT == GS_TYPE_F32 ? 4 : 2), i);
+    load4<VEC>(mu, i, m[u]);
+    load4<VEC>(nu, i, v[u]);
   }
   unsigned act = 0xFFFFFFFFu;
   if (d.active) {
-    // row of element e: (base + e) / width, by multiplications with the
-    // rounded-up reciprocal (exact: base < 2^37 and width <= 2^15, so that
-    // their product with the reciprocal's excess stays below its scale)
-    const unsigned w = d.width;
-    const unsigned long long row0 = w == 1 ? (unsigned long long)base : __umul64hi((unsigned long long)base, d.magic);
-    const unsigned rem0 = (unsigned)((unsigned long long)base - row0 * w);
-    const unsigned magic = (unsigned)(d.magic >> 32) + 1u;  // > 2^32 / width
-    const uint8_t* flags = d.active + row0;
-    act = 0u;
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const unsigned x = rem0 + u * kAdamwBlock + block_element<VEC>(lane, q);
-        const unsigned r = w == 1 ? x : __umulhi(x, magic);
-        act |= (flags[r] != 0 ? 1u : 0u) << (4 * u + q);
-      }
+    RowPlace rows;
+    rows.start(d, (unsigned long long)base);
+    act = active_bits<VEC, U>(d, rows, 0, lane);
   }
 #pragma unroll
   for (int u = 0; u < U; ++u) {
-    const long long b = base + u * kAdamwBlock;
-    float up_m = 0.f, up_v = 0.f;
-    if (BITS == 8) {
-      up_m = pow2_biased(min(fm[u], 254));
-      up_v = pow2_biased(min(fv[u], 254));
-      if (fm[u] == 255) up_m = NAN;
-      if (fv[u] == 255) up_v = NAN;
-    }
-    unsigned top_m = 0u, top_v = 0u;
+    const unsigned i = i0 + u * kAdamwBlock;
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
-      if (BITS == 8) {
-        m[u][q] = decode8<true>((cm[u] >> (8 * q)) & 255u, up_m);
-        v[u][q] = decode8<false>((cv[u] >> (8 * q)) & 255u, up_v);
-      }
       const float gq = g[u].get(q) * s;
       m[u][q] = add_rn(mul_rn(m[u][q], a.b1), mul_rn(gq, a.omb1));
       v[u][q] = add_rn(mul_rn(v[u][q], a.b2), mul_rn(mul_rn(gq, gq), a.omb2));
       const float fresh = adamw_param(p[u][q], m[u][q], v[u][q], h, a.eps);
       if ((act >> (4 * u + q)) & 1u) p[u][q] = fresh;
-      if (BITS == 8) {
-        top_m = max(top_m, __float_as_uint(fabsf(m[u][q])));
-        top_v = max(top_v, __float_as_uint(v[u][q]) & 0x7FFFFFFFu);
-      }
     }
-    store4<VEC>(d.param + b, lane, p[u]);
-    if (d.copy) store_copy4<VEC>(d.copy, b, lane, d.copy_type, p[u]);
-    if (BITS == 32) {
-      store4<VEC>(static_cast<float*>(d.mu) + b, lane, m[u]);
-      store4<VEC>(static_cast<float*>(d.nu) + b, lane, v[u]);
-    } else {
-      const int nm = block_field(__reduce_max_sync(0xffffffffu, top_m));
-      const int nv = block_field(__reduce_max_sync(0xffffffffu, top_v));
-      const float down_m = pow2_biased(max(254 - nm, 0)), down_v = pow2_biased(max(254 - nv, 0));
-      const unsigned bkey = mix32(key ^ (unsigned)(blk0 + u));
-      unsigned wm = 0u, wv = 0u;
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const unsigned r = mix32(bkey + kGolden * (unsigned)block_element<VEC>(lane, q));
-        wm |= encode8<true>(m[u][q], down_m, (r & 0xFFFFu) << 4) << (8 * q);
-        wv |= encode8<false>(v[u][q], down_v, (r >> 16) << 4) << (8 * q);
-      }
-      store_codes<VEC>(d.mu, b, lane, nm == 255 ? 0u : wm);
-      store_codes<VEC>(d.nu, b, lane, nv == 255 ? 0u : wv);
-      if (lane == 0) {
-        d.mu_exp[blk0 + u] = (uint8_t)nm;
-        d.nu_exp[blk0 + u] = (uint8_t)nv;
-      }
-    }
+    store4<VEC>(param, i, p[u]);
+    if (d.copy) store_copy4<VEC>(static_cast<char*>(d.copy) + base * 2, i, d.copy_type, p[u]);
+    store4<VEC>(mu, i, m[u]);
+    store4<VEC>(nu, i, v[u]);
   }
 }
 
-// One block of a tensor by one warp, `rem` elements of it in range.
+// The new moments of a block as codes and exponent bytes: fm, fv in and out.
+template <bool VEC>
+__device__ __forceinline__ void encode_block(const float m[4], const float v[4], float top_m, float top_v,
+                                             unsigned key, unsigned blk, int lane, unsigned& cm, unsigned& cv,
+                                             int& fm, int& fv) {
+  fm = block_field(__reduce_max_sync(0xffffffffu, __float_as_uint(top_m)));
+  fv = block_field(__reduce_max_sync(0xffffffffu, __float_as_uint(top_v)));
+  const unsigned bkey = mix32(key ^ blk) + kGolden * (unsigned)block_element<VEC>(lane, 0);
+  unsigned lo[4], hi[4];
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    const unsigned r = mix32(bkey + kGolden * (unsigned)block_element<VEC>(0, q));
+    lo[q] = (r << 4) & 0xFFFF0u;
+    hi[q] = (r >> 12) & 0xFFFF0u;
+  }
+  cm = encode4<true>(m, fm, lo);
+  cv = encode4<false>(v, fv, hi);
+}
+
+// Up to one block by one warp, `rem` elements of it in range, element by
+// element: the end of a tensor, and, with 8-bit moments, tensors whose
+// pointers are not 16-byte aligned.
 template <int BITS>
-__device__ __forceinline__ void adamw_block(const AdamwDesc& d, long long base, int rem, const AdamwParams& a,
-                                            const AdamwStep& h, float s, unsigned key) {
+__device__ __forceinline__ void adamw_rest(const AdamwDesc& d, long long base, int rem, const AdamwParams& a,
+                                           const AdamwStep& h, float s, unsigned key) {
   const int lane = threadIdx.x & 31;
   const long long blk = base / kAdamwBlock;
-  float p[4], m[4], v[4];
-  float up_m = 0.f, up_v = 0.f;
-  bool nan_m = false, nan_v = false;
-  if (BITS == 8) {
-    const int fm = d.mu_exp[blk], fv = d.nu_exp[blk];
-    nan_m = fm == 255;
-    nan_v = fv == 255;
-    up_m = pow2_biased(min(fm, 254));
-    up_v = pow2_biased(min(fv, 254));
+  RowPlace rows;
+  if (d.active) rows.start(d, (unsigned long long)base);
+  float p[4], g[4], m[4], v[4];
+  float top_m = 0.f, top_v = 0.f;
+  unsigned cm = 0u, cv = 0u, act = 0u;
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    p[q] = g[q] = m[q] = v[q] = 0.f;
+    const int e = lane + 32 * q;
+    const long long i = base + e;
+    if (e >= rem) continue;
+    p[q] = d.param[i];
+    g[q] = load_as_float(d.grad, i, d.grad_type) * s;
+    if (BITS == 8) {
+      cm |= (unsigned)static_cast<const uint8_t*>(d.mu)[i] << (8 * q);
+      cv |= (unsigned)static_cast<const uint8_t*>(d.nu)[i] << (8 * q);
+    } else {
+      m[q] = mul_rn(static_cast<const float*>(d.mu)[i], a.b1);
+      v[q] = mul_rn(static_cast<const float*>(d.nu)[i], a.b2);
+    }
+    if (!d.active || rows.flags[RowPlace::rows(d, rows.rest + e)] != 0) act |= 1u << q;
   }
-  unsigned top_m = 0u, top_v = 0u;
+  if (BITS == 8) {
+    decayed4<true>(cm, d.mu_exp[blk], a.b1, m);
+    decayed4<false>(cv, d.nu_exp[blk], a.b2, v);
+  }
 #pragma unroll
   for (int q = 0; q < 4; ++q) {
     const int e = lane + 32 * q;
     const long long i = base + e;
-    p[q] = m[q] = v[q] = 0.f;
-    if (e >= rem) continue;
-    float g = load_as_float(d.grad, i, d.grad_type) * s;
-    p[q] = d.param[i];
-    if (BITS == 8) {
-      m[q] = decode8<true>(static_cast<const uint8_t*>(d.mu)[i], up_m);
-      v[q] = decode8<false>(static_cast<const uint8_t*>(d.nu)[i], up_v);
-      if (nan_m) m[q] = NAN;
-      if (nan_v) v[q] = NAN;
-    } else {
-      m[q] = static_cast<const float*>(d.mu)[i];
-      v[q] = static_cast<const float*>(d.nu)[i];
+    if (e >= rem) {
+      m[q] = v[q] = 0.f;
+      continue;
     }
-    m[q] = add_rn(mul_rn(m[q], a.b1), mul_rn(g, a.omb1));
-    v[q] = add_rn(mul_rn(v[q], a.b2), mul_rn(mul_rn(g, g), a.omb2));
-    const float fresh = adamw_param(p[q], m[q], v[q], h, a.eps);
-    if (!d.active || d.active[i / d.width] != 0) {
-      p[q] = fresh;
-      d.param[i] = fresh;
+    m[q] = add_rn(m[q], mul_rn(g[q], a.omb1));
+    v[q] = add_rn(v[q], mul_rn(mul_rn(g[q], g[q]), a.omb2));
+    if ((act >> q) & 1u) {
+      p[q] = adamw_param(p[q], m[q], v[q], h, a.eps);
+      d.param[i] = p[q];
     }
     if (d.copy) store_as(d.copy, i, d.copy_type, p[q]);
     if (BITS == 32) {
       static_cast<float*>(d.mu)[i] = m[q];
       static_cast<float*>(d.nu)[i] = v[q];
     }
-    top_m = max(top_m, __float_as_uint(fabsf(m[q])));
-    top_v = max(top_v, __float_as_uint(fabsf(v[q])));
+    top_m = max_abs(top_m, m[q]);
+    top_v = max_abs(top_v, v[q]);
   }
-  if (BITS == 8) {
-    const int fm = block_field(__reduce_max_sync(0xffffffffu, top_m));
-    const int fv = block_field(__reduce_max_sync(0xffffffffu, top_v));
-    const float down_m = pow2_biased(max(254 - fm, 0)), down_v = pow2_biased(max(254 - fv, 0));
-    const unsigned bkey = mix32(key ^ (unsigned)blk);
+  if (BITS == 32) return;
+  int fm, fv;
+  encode_block<false>(m, v, top_m, top_v, key, (unsigned)blk, lane, cm, cv, fm, fv);
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const int e = lane + 32 * q;
-      if (e >= rem) continue;
-      const unsigned r = mix32(bkey + kGolden * (unsigned)e);
-      unsigned cm = encode8<true>(m[q], down_m, (r & 0xFFFFu) << 4);
-      unsigned cv = encode8<false>(v[q], down_v, (r >> 16) << 4);
-      if (fm == 255) cm = 0u;
-      if (fv == 255) cv = 0u;
-      static_cast<uint8_t*>(d.mu)[base + e] = (uint8_t)cm;
-      static_cast<uint8_t*>(d.nu)[base + e] = (uint8_t)cv;
-    }
-    if (lane == 0) {
-      d.mu_exp[blk] = (uint8_t)fm;
-      d.nu_exp[blk] = (uint8_t)fv;
-    }
+  for (int q = 0; q < 4; ++q) {
+    const int e = lane + 32 * q;
+    if (e >= rem) continue;
+    static_cast<uint8_t*>(d.mu)[base + e] = (uint8_t)(cm >> (8 * q));
+    static_cast<uint8_t*>(d.nu)[base + e] = (uint8_t)(cv >> (8 * q));
+  }
+  if (lane == 0) {
+    d.mu_exp[blk] = (uint8_t)fm;
+    d.nu_exp[blk] = (uint8_t)fv;
   }
 }
 
-template <int BITS, int N>
-__global__ void __launch_bounds__(32 * kAdamwWarps)
-k_adamw(const __grid_constant__ AdamwTable<N> tab, const __grid_constant__ AdamwParams a) {
-  GS_PDL_ENTRY_PLAIN();
-  const int c = *(volatile int*)a.state;
-  const float s = a.scale ? *(volatile const float*)a.scale : 1.f;
-  const bool go = fabsf(s) <= 3.402823466e38f;
-  if (go) {
-    const float cf = (float)c;
-    AdamwStep h;
-    // 1 - b^t as -expm1(t ln b): no cancellation at small t
-    h.inv1 = 1.f / -expm1f((cf + 1.f) * a.ln_b1);
-    h.inv2 = 1.f / -expm1f((cf + 1.f) * a.ln_b2);
-    const unsigned key = mix32(a.seed + kGolden * (unsigned)c);
-    const int tiles = tab.first[tab.n];
-    int k = 0;
-    for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
-      // the last tensor whose first tile is not behind this one
-      int hi = tab.n;
-      while (hi - k > 1) {
-        const int mid = (k + hi) >> 1;
-        if (tab.first[mid] <= tile) k = mid;
-        else hi = mid;
-      }
-      const AdamwDesc& d = tab.t[k];
-      h.lr = d.lr_init * expf(cf * d.ln_decay);
-      h.wd = d.weight_decay;
-      const long long base = (long long)(tile - tab.first[k]) * kAdamwTile + (threadIdx.x >> 5) * kAdamwChunk;
-      const long long left = d.count - base;
-      if (left <= 0) continue;
-      const unsigned tkey = mix32(key + kGolden * (unsigned)(tab.index0 + k));
-      if (left >= kAdamwChunk) {
-        switch (d.grad_type * 2 + d.vec) {
-          case 0: adamw_chunk<BITS, GS_TYPE_F32, false>(d, base, a, h, s, tkey); break;
-          case 1: adamw_chunk<BITS, GS_TYPE_F32, true>(d, base, a, h, s, tkey); break;
-          case 2: adamw_chunk<BITS, GS_TYPE_BF16, false>(d, base, a, h, s, tkey); break;
-          case 3: adamw_chunk<BITS, GS_TYPE_BF16, true>(d, base, a, h, s, tkey); break;
-          case 4: adamw_chunk<BITS, GS_TYPE_F16, false>(d, base, a, h, s, tkey); break;
-          default: adamw_chunk<BITS, GS_TYPE_F16, true>(d, base, a, h, s, tkey); break;
-        }
-      } else {
-        for (int e = 0; e < left; e += kAdamwBlock)
-          adamw_block<BITS>(d, base + e, (int)(left - e < kAdamwBlock ? left - e : kAdamwBlock), a, h, s, tkey);
-      }
-    }
-  }
-  if (!a.advance) return;
-  // the last CTA to finish (atomic ticket, no waiting) advances the count
+// The last CTA to finish (atomic ticket, no waiting) advances the count.
+__device__ __forceinline__ void adamw_advance(const AdamwParams& a, int c, bool go) {
   __syncthreads();
   if (threadIdx.x == 0) {
     __threadfence();
@@ -466,6 +495,231 @@ k_adamw(const __grid_constant__ AdamwTable<N> tab, const __grid_constant__ Adamw
       a.state[1] = 0;
     }
   }
+}
+
+// A CTA's walk over the tiles of a table, every gridDim.x-th.
+template <int N>
+struct TileWalk {
+  const AdamwTable<N>& tab;
+  int tile, k;
+
+  __device__ __forceinline__ TileWalk(const AdamwTable<N>& t) : tab(t), tile(blockIdx.x), k(0) {
+    // the last tensor whose first tile is not behind this one
+    for (int hi = tab.n; hi - k > 1;) {
+      const int mid = (k + hi) >> 1;
+      if (tab.first[mid] <= tile) k = mid;
+      else hi = mid;
+    }
+  }
+  __device__ __forceinline__ bool valid() const { return tile < tab.first[tab.n]; }
+  __device__ __forceinline__ void next() {
+    tile += gridDim.x;
+    if (valid())
+      while (tab.first[k + 1] <= tile) ++k;
+  }
+  // first element of this warp's chunk
+  __device__ __forceinline__ long long base() const {
+    return (long long)(tile - tab.first[k]) * kAdamwTile + (threadIdx.x >> 5) * kAdamwChunk;
+  }
+};
+
+// Step values of a tensor. 1 - b^t as -expm1(t ln b): no cancellation at small t.
+__device__ __forceinline__ void adamw_bias(AdamwStep& h, const AdamwParams& a, float cf) {
+  h.inv1 = 1.f / -expm1f((cf + 1.f) * a.ln_b1);
+  h.inv2 = 1.f / -expm1f((cf + 1.f) * a.ln_b2);
+}
+__device__ __forceinline__ void adamw_rates(AdamwStep& h, const AdamwDesc& d, float cf) {
+  h.lr = d.lr_init * expf(cf * d.ln_decay);
+  h.wd = d.weight_decay;
+}
+
+template <int N>
+__global__ void __launch_bounds__(32 * kAdamwWarps, GS_ADAMW_CTAS)
+k_adamw32(const __grid_constant__ AdamwTable<N> tab, const __grid_constant__ AdamwParams a) {
+  GS_PDL_ENTRY_PLAIN();
+  const int c = *(volatile int*)a.state;
+  const float s = a.scale ? *(volatile const float*)a.scale : 1.f;
+  const bool go = fabsf(s) <= 3.402823466e38f;
+  if (go) {
+    AdamwStep h;
+    adamw_bias(h, a, (float)c);
+    int last = -1;
+    for (TileWalk<N> w(tab); w.valid(); w.next()) {
+      const AdamwDesc& d = tab.t[w.k];
+      if (w.k != last) adamw_rates(h, d, (float)c);
+      last = w.k;
+      const long long base = w.base(), left = d.count - base;
+      if (left >= kAdamwChunk) {
+        switch (d.grad_type * 2 + d.vec) {
+          case 0: adamw32_chunk<GS_TYPE_F32, false>(d, base, a, h, s); break;
+          case 1: adamw32_chunk<GS_TYPE_F32, true>(d, base, a, h, s); break;
+          case 2: adamw32_chunk<GS_TYPE_BF16, false>(d, base, a, h, s); break;
+          case 3: adamw32_chunk<GS_TYPE_BF16, true>(d, base, a, h, s); break;
+          case 4: adamw32_chunk<GS_TYPE_F16, false>(d, base, a, h, s); break;
+          default: adamw32_chunk<GS_TYPE_F16, true>(d, base, a, h, s); break;
+        }
+      } else {
+        for (int e = 0; e < left; e += kAdamwBlock)
+          adamw_rest<32>(d, base + e, (int)(left - e < kAdamwBlock ? left - e : kAdamwBlock), a, h, s, 0u);
+      }
+    }
+  }
+  if (a.advance) adamw_advance(a, c, go);
+}
+
+// 8-bit moments. The step costs some 70 instructions an element, about what
+// the SMs can issue in the time that its bytes take, so no warp may wait for
+// memory: each copies its next chunk into shared memory (cp.async, 16 bytes
+// a lane) before it works on the current one.
+struct __align__(16) Adamw8Stage {
+  float p[kAdamwChunk];
+  unsigned g[kAdamwChunk];
+  uint8_t mu[kAdamwChunk], nu[kAdamwChunk];
+};
+
+__device__ __forceinline__ void cp_async16(void* dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((unsigned)__cvta_generic_to_shared(dst)), "l"(src)
+               : "memory");
+}
+
+// A chunk on its way: what the copies do not carry.
+struct Adamw8Chunk {
+  long long base;
+  int k;
+  bool piped;     // copied to shared memory
+  unsigned act;   // flags of the lane's elements
+  unsigned exps;  // exponent byte of mu (lanes 0, 1) or nu (2, 3) of block lane & 1
+};
+
+__device__ __forceinline__ void adamw8_issue(const AdamwDesc& d, Adamw8Chunk& c, Adamw8Stage& st, int lane) {
+  c.piped = d.vec && d.count - c.base >= kAdamwChunk;
+  if (c.piped) {
+    const char* p = reinterpret_cast<const char*>(d.param + c.base) + 16 * lane;
+    cp_async16(reinterpret_cast<char*>(st.p) + 16 * lane, p);
+    cp_async16(reinterpret_cast<char*>(st.p) + 16 * lane + 512, p + 512);
+    const char* g = static_cast<const char*>(d.grad) + (c.base << (d.grad_type == GS_TYPE_F32 ? 2 : 1)) + 16 * lane;
+    cp_async16(reinterpret_cast<char*>(st.g) + 16 * lane, g);
+    if (d.grad_type == GS_TYPE_F32) cp_async16(reinterpret_cast<char*>(st.g) + 16 * lane + 512, g + 512);
+    const uint8_t* m = static_cast<const uint8_t*>(lane < 16 ? d.mu : d.nu) + c.base + 16 * (lane & 15);
+    cp_async16((lane < 16 ? st.mu : st.nu) + 16 * (lane & 15), m);
+    c.exps = lane < 4 ? (lane < 2 ? d.mu_exp : d.nu_exp)[c.base / kAdamwBlock + (lane & 1)] : 0u;
+    c.act = 0xFFFFFFFFu;
+    if (d.active) {
+      RowPlace rows;
+      rows.start(d, (unsigned long long)c.base);
+      c.act = active_bits<true, kAdamwUnroll>(d, rows, 0, lane);
+    }
+  }
+  asm volatile("cp.async.commit_group;" ::: "memory");
+}
+
+__device__ __forceinline__ void adamw8_chunk(const AdamwDesc& d, const Adamw8Chunk& c, const Adamw8Stage& st,
+                                             const AdamwParams& a, const AdamwStep& h, float s, unsigned key, int lane) {
+  constexpr int U = kAdamwUnroll;
+  const unsigned blk0 = (unsigned)(c.base / kAdamwBlock);
+  float* const param = d.param + c.base;
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const unsigned i = u * kAdamwBlock + 4 * lane;
+    float p[4], g[4], m[4], v[4], fresh[4];
+    load4<true>(st.p, i, p);
+    if (d.grad_type == GS_TYPE_F32) {
+      load4<true>(reinterpret_cast<const float*>(st.g), i, g);
+    } else {
+      const uint2 w = *reinterpret_cast<const uint2*>(reinterpret_cast<const uint16_t*>(st.g) + i);
+      const unsigned x[4] = {w.x << 16, w.x & 0xFFFF0000u, w.y << 16, w.y & 0xFFFF0000u};
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        g[q] = d.grad_type == GS_TYPE_BF16 ? __uint_as_float(x[q])
+                                           : __half2float(__ushort_as_half((unsigned short)(x[q] >> 16)));
+    }
+    unsigned cm = load_codes<true>(st.mu, i), cv = load_codes<true>(st.nu, i);
+    int fm = (int)__shfl_sync(0xffffffffu, c.exps, u), fv = (int)__shfl_sync(0xffffffffu, c.exps, 2 + u);
+    decayed4<true>(cm, fm, a.b1, m);
+    decayed4<false>(cv, fv, a.b2, v);
+    float top_m = 0.f, top_v = 0.f;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const float gq = g[q] * s;
+      m[q] = add_rn(m[q], mul_rn(gq, a.omb1));
+      v[q] = add_rn(v[q], mul_rn(mul_rn(gq, gq), a.omb2));
+      fresh[q] = adamw_param(p[q], m[q], v[q], h, a.eps);
+      top_m = max_abs(top_m, m[q]);
+      top_v = max_abs(top_v, v[q]);
+    }
+    const unsigned act = (c.act >> (4 * u)) & 15u;
+    if (!__all_sync(0xffffffffu, act == 15u)) {
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        if (!((act >> q) & 1u)) fresh[q] = p[q];
+    }
+    store4<true>(param, i, fresh);
+    if (d.copy) store_copy4<true>(static_cast<char*>(d.copy) + c.base * 2, i, d.copy_type, fresh);
+    encode_block<true>(m, v, top_m, top_v, key, blk0 + u, lane, cm, cv, fm, fv);
+    store_codes<true>(static_cast<uint8_t*>(d.mu) + c.base, i, cm);
+    store_codes<true>(static_cast<uint8_t*>(d.nu) + c.base, i, cv);
+    if (lane == 0) {
+      (d.mu_exp + c.base / kAdamwBlock)[u] = (uint8_t)fm;
+      (d.nu_exp + c.base / kAdamwBlock)[u] = (uint8_t)fv;
+    }
+  }
+}
+
+template <int N>
+__global__ void __launch_bounds__(32 * kAdamwWarps, GS_ADAMW8_CTAS)
+k_adamw8(const __grid_constant__ AdamwTable<N> tab, const __grid_constant__ AdamwParams a) {
+  GS_PDL_ENTRY_PLAIN();
+  __shared__ Adamw8Stage stages[kAdamwWarps][2];
+  const int c = *(volatile int*)a.state;
+  const float s = a.scale ? *(volatile const float*)a.scale : 1.f;
+  const bool go = fabsf(s) <= 3.402823466e38f;
+  if (go) {
+    const int lane = threadIdx.x & 31;
+    AdamwStep h;
+    adamw_bias(h, a, (float)c);
+    const unsigned key = mix32(a.seed + kGolden * (unsigned)c);
+    unsigned tkey = 0u;
+    TileWalk<N> w(tab);
+    Adamw8Chunk now, next;
+    Adamw8Stage* st = stages[threadIdx.x >> 5];
+    int at = 0, last = -1;
+    bool more = w.valid();
+    if (more) {
+      now.k = w.k;
+      now.base = w.base();
+      adamw8_issue(tab.t[now.k], now, st[0], lane);
+    }
+    while (more) {
+      w.next();
+      more = w.valid();
+      if (more) {
+        next.k = w.k;
+        next.base = w.base();
+        adamw8_issue(tab.t[next.k], next, st[at ^ 1], lane);
+        asm volatile("cp.async.wait_group 1;" ::: "memory");
+      } else {
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+      }
+      __syncwarp();
+      const AdamwDesc& d = tab.t[now.k];
+      if (now.k != last) {
+        adamw_rates(h, d, (float)c);
+        tkey = mix32(key + kGolden * (unsigned)(tab.index0 + now.k));
+        last = now.k;
+      }
+      if (now.piped) {
+        adamw8_chunk(d, now, st[at], a, h, s, tkey, lane);
+      } else {
+        const long long left = d.count - now.base;
+        for (int e = 0; e < kAdamwChunk && e < left; e += kAdamwBlock)
+          adamw_rest<8>(d, now.base + e, (int)(left - e < kAdamwBlock ? left - e : kAdamwBlock), a, h, s, tkey);
+      }
+      __syncwarp();  // the stage has been read before it is copied into again
+      now = next;
+      at ^= 1;
+    }
+  }
+  if (a.advance) adamw_advance(a, c, go);
 }
 
 template <int BITS, int N>
@@ -491,8 +745,8 @@ static void launch_adamw_class(const GsAdamwTensor* t, int n, int index0, const 
     d.copy_type = (uint8_t)t[i].copy_type;
     d.magic = t[i].width > 1 ? ~0ull / (unsigned)t[i].width + 1ull : 0ull;
     const size_t g4 = t[i].grad_type == GS_TYPE_F32 ? 16 : 8;
-    uintptr_t bits = (uintptr_t)t[i].param | ((uintptr_t)t[i].copy * 2) | ((uintptr_t)t[i].grad * (16 / g4));
-    if (BITS == 32) bits |= (uintptr_t)t[i].mu | (uintptr_t)t[i].nu;
+    uintptr_t bits = (uintptr_t)t[i].param | ((uintptr_t)t[i].copy * 2) | ((uintptr_t)t[i].grad * (BITS == 8 ? 1 : 16 / g4));
+    bits |= (uintptr_t)t[i].mu | (uintptr_t)t[i].nu;
     d.vec = (bits & 15) == 0;
     tab.first[i] = tiles;
     tiles += (int)((t[i].count + kAdamwTile - 1) / kAdamwTile);
@@ -500,9 +754,9 @@ static void launch_adamw_class(const GsAdamwTensor* t, int n, int index0, const 
   tab.first[n] = tiles;
   tab.n = n;
   tab.index0 = index0;
-  const int grid = std::max(1, std::min(tiles, device_sms() * 8));
+  const int grid = std::max(1, std::min(tiles, device_sms() * (BITS == 8 ? GS_ADAMW8_CTAS : 8)));
   GS_TIMED(BITS == 8 ? "adamw8" : "adamw", st);
-  launch_kernel_plain(k_adamw<BITS, N>, grid, 32 * kAdamwWarps, 0, st, tab, a);
+  launch_kernel_plain(BITS == 8 ? k_adamw8<N> : k_adamw32<N>, grid, 32 * kAdamwWarps, 0, st, tab, a);
 }
 
 constexpr int kAdamwSmall = 8, kAdamwMost = 256;

@@ -685,7 +685,7 @@ int gs_adamw_step(const GsAdamwTensor* tensors, int n_tensors, const GsAdamwConf
   if (config->moment_bits != 32 && config->moment_bits != 8) return GS_ERR_INVALID_ARGUMENT;
   if (!(config->b1 >= 0.0 && (float)config->b1 < 1.f) || !(config->b2 >= 0.0 && (float)config->b2 < 1.f))
     return GS_ERR_INVALID_ARGUMENT;
-  if (!((float)config->eps > 0.f) || !std::isfinite((float)config->eps)) return GS_ERR_INVALID_ARGUMENT;
+  if (!((float)config->eps >= 1.17549435e-38f) || !std::isfinite((float)config->eps)) return GS_ERR_INVALID_ARGUMENT;
   int64_t tiles = 0;
   for (int i = 0; i < n_tensors; ++i) {
     if (int s = check_adamw_tensor(tensors[i], config->moment_bits)) return s;

@@ -50,7 +50,7 @@ def test_step_refuses_tensors(kw):
 
 
 @pytest.mark.parametrize("kw", [dict(moment_bits=16), dict(b1=1.0), dict(b1=-0.1), dict(b2=1.0), dict(b2=math.nan),
-                                dict(b2=1.0 - 1e-12), dict(eps=0.0), dict(eps=1e-60), dict(eps=math.inf),
+                                dict(b2=1.0 - 1e-12), dict(eps=0.0), dict(eps=1e-60), dict(eps=1e-39), dict(eps=math.inf),
                                 dict(eps=math.nan)])
 def test_step_refuses_hyperparameters(kw):
     assert step(c=config(**kw)) == E
