@@ -83,6 +83,7 @@ struct AdamwTable {
 struct AdamwParams {
   float b1, omb1, b2, omb2, eps, ln_b1, ln_b2;
   unsigned seed;
+  bool fine_root;  // eps is so small that the root of a subnormal v counts beside it
   const float* scale;
   int* state;    // [count, ticket, skipped, 0]
   bool advance;  // this launch is the step's last
@@ -135,22 +136,38 @@ __device__ __forceinline__ void store_as(void* p, long long i, int type, float x
 }
 
 struct AdamwStep {
-  float lr, wd, inv1, inv2;
+  float inv1, inv2;   // 1 / (1 - b^t)
+  float rate, decay;  // lr inv1 and -lr wd of the tensor
 };
 
-// eps is a normal float, so the denominator is one and lies far below 2^126:
-// the reciprocal needs no care for subnormals (the square root does).
-__device__ __forceinline__ float adamw_param(float p, float m, float v, const AdamwStep& h, float eps) {
-  float root, inv;
-  asm("sqrt.approx.f32 %0, %1;" : "=f"(root) : "f"(v * h.inv2));
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(root + eps));
-  return p - h.lr * ((m * h.inv1) * inv + h.wd * p);
+// p - lr (m inv1 / (sqrt(v inv2) + eps) + wd p) for four elements. eps is a
+// normal float, so the denominator is one too and lies far below 2^126: the
+// approximate reciprocal needs no care for subnormals. The root of a
+// subnormal is below 2^-63; as 0 it changes a denominator by less than a
+// rounding unless eps < 2^-39.
+__device__ __forceinline__ void adamw_param4(const float p[4], const float m[4], const float v[4], const AdamwStep& h,
+                                             const AdamwParams& a, float out[4]) {
+  float root[4];
+  if (a.fine_root) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) asm("sqrt.approx.f32 %0, %1;" : "=f"(root[q]) : "f"(v[q] * h.inv2));
+  } else {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(root[q]) : "f"(v[q] * h.inv2));
+  }
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    float inv;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(root[q] + a.eps));
+    out[q] = fmaf(-(m[q] * h.rate), inv, fmaf(h.decay, p[q], p[q]));
+  }
 }
 
-// max(a, |b|), NaN if one is
-__device__ __forceinline__ float max_abs(float a, float b) {
+// Largest magnitude of four, NaN if one is.
+__device__ __forceinline__ float max_abs4(const float x[4]) {
   float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(fabsf(b)));
+  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(x[0]), "f"(x[1]), "f"(x[2]));
+  asm("max.NaN.abs.f32 %0, %1, %2, %2;" : "=f"(r) : "f"(r), "f"(x[3]));
   return r;
 }
 
@@ -182,6 +199,13 @@ __device__ __forceinline__ void store4(float* p, unsigned i, const float x[4]) {
 #pragma unroll
     for (int q = 0; q < 4; ++q) p[i + 32 * q] = x[q];
   }
+}
+
+__device__ __forceinline__ bool differ4(const float x[4], const float y[4]) {
+  unsigned d = 0u;
+#pragma unroll
+  for (int q = 0; q < 4; ++q) d |= __float_as_uint(x[q]) ^ __float_as_uint(y[q]);
+  return d != 0u;
 }
 
 // Four gradients as loaded (16-bit ones two to a register where VEC).
@@ -314,37 +338,23 @@ __device__ __forceinline__ void decayed4(unsigned w, int field, float b, float x
   }
 }
 
-// encode8 of four values under their block's exponent byte, one code a byte.
-// The scale is a single power of two while 2^(127 - F) 2^-112 or 2^-96 is a
-// normal float. No code exceeds the largest: F leaves the largest magnitude
-// at most at the top code, and noise is less than the next code away.
+// encode8 of four values that `scale` takes to their block's format, one code
+// a byte. No code exceeds the largest: F leaves the largest magnitude at most
+// at the top code, and noise is less than the next code away.
 template <bool SIGNED>
-__device__ __forceinline__ unsigned encode4(const float x[4], int field, const unsigned noise[4]) {
-  constexpr int kShift = SIGNED ? 15 : 31;
-  float scale, z[4] = {x[0], x[1], x[2], x[3]};
-  if (field <= 126 + kShift) {
-    scale = __int_as_float((127 + kShift - field) << 23);
-  } else {
-    const float first = pow2_biased(max(254 - field, 0));
-#pragma unroll
-    for (int q = 0; q < 4; ++q) z[q] *= first;
-    scale = SIGNED ? 0x1p-112f : 0x1p-96f;
-  }
+__device__ __forceinline__ unsigned encode4(const float x[4], float scale, const unsigned noise[4]) {
   unsigned c[4];
 #pragma unroll
   for (int q = 0; q < 4; ++q) {
-    const float y = z[q] * scale;
+    unsigned t = __float_as_uint(x[q] * scale) + noise[q];
     if (SIGNED) {
-      const unsigned t = __float_as_uint(y) + noise[q];
       c[q] = ((t << 4) & 0x7FFFFFFFu) | (t & 0x80000000u);
     } else {
-      unsigned t = __float_as_uint(y) + noise[q];
       if (x[q] > 0.f) t = max(t, 1u << 20);
       c[q] = t << 4;
     }
   }
-  const unsigned w = __byte_perm(__byte_perm(c[0], c[1], 0x0073), __byte_perm(c[2], c[3], 0x0073), 0x5410);
-  return field == 255 ? 0u : w;
+  return __byte_perm(__byte_perm(c[0], c[1], 0x0073), __byte_perm(c[2], c[3], 0x0073), 0x5410);
 }
 
 // Whole blocks with 32-bit moments from element `base` by one warp, all loads
@@ -377,28 +387,46 @@ __device__ __forceinline__ void adamw32_chunk(const AdamwDesc& d, long long base
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     const unsigned i = i0 + u * kAdamwBlock;
+    float m1[4], v1[4], p1[4];
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
       const float gq = g[u].get(q) * s;
-      m[u][q] = add_rn(mul_rn(m[u][q], a.b1), mul_rn(gq, a.omb1));
-      v[u][q] = add_rn(mul_rn(v[u][q], a.b2), mul_rn(mul_rn(gq, gq), a.omb2));
-      const float fresh = adamw_param(p[u][q], m[u][q], v[u][q], h, a.eps);
-      if ((act >> (4 * u + q)) & 1u) p[u][q] = fresh;
+      m1[q] = add_rn(mul_rn(m[u][q], a.b1), mul_rn(gq, a.omb1));
+      v1[q] = add_rn(mul_rn(v[u][q], a.b2), mul_rn(mul_rn(gq, gq), a.omb2));
     }
-    store4<VEC>(param, i, p[u]);
-    if (d.copy) store_copy4<VEC>(static_cast<char*>(d.copy) + base * 2, i, d.copy_type, p[u]);
-    store4<VEC>(mu, i, m[u]);
-    store4<VEC>(nu, i, v[u]);
+    adamw_param4(p[u], m1, v1, h, a, p1);
+    const unsigned bits = (act >> (4 * u)) & 15u;
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      if (!((bits >> q) & 1u)) p1[q] = p[u][q];
+    if (d.copy) store_copy4<VEC>(static_cast<char*>(d.copy) + base * 2, i, d.copy_type, p1);
+    // what did not change (masked rows; slots that never had a gradient) is not stored again
+    if (bits != 0u) store4<VEC>(param, i, p1);
+    if (differ4(m1, m[u])) store4<VEC>(mu, i, m1);
+    if (differ4(v1, v[u])) store4<VEC>(nu, i, v1);
   }
 }
 
-// The new moments of a block as codes and exponent bytes: fm, fv in and out.
+// The new moments of a block as codes and exponent bytes (fm, fv out). The
+// scales are powers of two, 2^(127 - F) 2^-112 and 2^-96, as long as those are
+// normal floats; beyond, in two steps.
 template <bool VEC>
-__device__ __forceinline__ void encode_block(const float m[4], const float v[4], float top_m, float top_v,
-                                             unsigned key, unsigned blk, int lane, unsigned& cm, unsigned& cv,
-                                             int& fm, int& fv) {
-  fm = block_field(__reduce_max_sync(0xffffffffu, __float_as_uint(top_m)));
-  fv = block_field(__reduce_max_sync(0xffffffffu, __float_as_uint(top_v)));
+__device__ __forceinline__ void encode_block(float m[4], float v[4], unsigned key, unsigned blk, int lane,
+                                             unsigned& cm, unsigned& cv, int& fm, int& fv) {
+  fm = block_field(__reduce_max_sync(0xffffffffu, __float_as_uint(max_abs4(m))));
+  fv = block_field(__reduce_max_sync(0xffffffffu, __float_as_uint(max_abs4(v))));
+  float sm = __int_as_float((142 - fm) << 23), sv = __int_as_float((158 - fv) << 23);
+  if (fm > 141 || fv > 157) {
+    const float dm = pow2_biased(max(254 - fm, 0)), dv = pow2_biased(max(254 - fv, 0));
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      m[q] = fm == 255 ? 0.f : m[q] * dm;
+      // a v > 0 stays above 0
+      v[q] = fv == 255 ? 0.f : (v[q] > 0.f ? fmaxf(v[q] * dv, __int_as_float(1)) : 0.f);
+    }
+    sm = 0x1p-112f;
+    sv = 0x1p-96f;
+  }
   const unsigned bkey = mix32(key ^ blk) + kGolden * (unsigned)block_element<VEC>(lane, 0);
   unsigned lo[4], hi[4];
 #pragma unroll
@@ -407,8 +435,8 @@ __device__ __forceinline__ void encode_block(const float m[4], const float v[4],
     lo[q] = (r << 4) & 0xFFFF0u;
     hi[q] = (r >> 12) & 0xFFFF0u;
   }
-  cm = encode4<true>(m, fm, lo);
-  cv = encode4<false>(v, fv, hi);
+  cm = encode4<true>(m, sm, lo);
+  cv = encode4<false>(v, sv, hi);
 }
 
 // Up to one block by one warp, `rem` elements of it in range, element by
@@ -422,7 +450,6 @@ __device__ __forceinline__ void adamw_rest(const AdamwDesc& d, long long base, i
   RowPlace rows;
   if (d.active) rows.start(d, (unsigned long long)base);
   float p[4], g[4], m[4], v[4];
-  float top_m = 0.f, top_v = 0.f;
   unsigned cm = 0u, cv = 0u, act = 0u;
 #pragma unroll
   for (int q = 0; q < 4; ++q) {
@@ -445,31 +472,28 @@ __device__ __forceinline__ void adamw_rest(const AdamwDesc& d, long long base, i
     decayed4<true>(cm, d.mu_exp[blk], a.b1, m);
     decayed4<false>(cv, d.nu_exp[blk], a.b2, v);
   }
+  float fresh[4];
 #pragma unroll
   for (int q = 0; q < 4; ++q) {
-    const int e = lane + 32 * q;
-    const long long i = base + e;
-    if (e >= rem) {
-      m[q] = v[q] = 0.f;
-      continue;
-    }
-    m[q] = add_rn(m[q], mul_rn(g[q], a.omb1));
-    v[q] = add_rn(v[q], mul_rn(mul_rn(g[q], g[q]), a.omb2));
-    if ((act >> q) & 1u) {
-      p[q] = adamw_param(p[q], m[q], v[q], h, a.eps);
-      d.param[i] = p[q];
-    }
+    const bool in = lane + 32 * q < rem;  // else zeros, which leave no trace in the block
+    m[q] = in ? add_rn(m[q], mul_rn(g[q], a.omb1)) : 0.f;
+    v[q] = in ? add_rn(v[q], mul_rn(mul_rn(g[q], g[q]), a.omb2)) : 0.f;
+  }
+  adamw_param4(p, m, v, h, a, fresh);
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    const long long i = base + lane + 32 * q;
+    if (lane + 32 * q >= rem) continue;
+    if ((act >> q) & 1u) d.param[i] = p[q] = fresh[q];
     if (d.copy) store_as(d.copy, i, d.copy_type, p[q]);
     if (BITS == 32) {
       static_cast<float*>(d.mu)[i] = m[q];
       static_cast<float*>(d.nu)[i] = v[q];
     }
-    top_m = max_abs(top_m, m[q]);
-    top_v = max_abs(top_v, v[q]);
   }
   if (BITS == 32) return;
   int fm, fv;
-  encode_block<false>(m, v, top_m, top_v, key, (unsigned)blk, lane, cm, cv, fm, fv);
+  encode_block<false>(m, v, key, (unsigned)blk, lane, cm, cv, fm, fv);
 #pragma unroll
   for (int q = 0; q < 4; ++q) {
     const int e = lane + 32 * q;
@@ -517,10 +541,8 @@ struct TileWalk {
     if (valid())
       while (tab.first[k + 1] <= tile) ++k;
   }
-  // first element of this warp's chunk
-  __device__ __forceinline__ long long base() const {
-    return (long long)(tile - tab.first[k]) * kAdamwTile + (threadIdx.x >> 5) * kAdamwChunk;
-  }
+  // first element of the tile in its tensor
+  __device__ __forceinline__ long long base() const { return (long long)(tile - tab.first[k]) * kAdamwTile; }
 };
 
 // Step values of a tensor. 1 - b^t as -expm1(t ln b): no cancellation at small t.
@@ -529,8 +551,9 @@ __device__ __forceinline__ void adamw_bias(AdamwStep& h, const AdamwParams& a, f
   h.inv2 = 1.f / -expm1f((cf + 1.f) * a.ln_b2);
 }
 __device__ __forceinline__ void adamw_rates(AdamwStep& h, const AdamwDesc& d, float cf) {
-  h.lr = d.lr_init * expf(cf * d.ln_decay);
-  h.wd = d.weight_decay;
+  const float lr = d.lr_init * expf(cf * d.ln_decay);
+  h.rate = lr * h.inv1;
+  h.decay = -lr * d.weight_decay;
 }
 
 template <int N>
@@ -548,7 +571,7 @@ k_adamw32(const __grid_constant__ AdamwTable<N> tab, const __grid_constant__ Ada
       const AdamwDesc& d = tab.t[w.k];
       if (w.k != last) adamw_rates(h, d, (float)c);
       last = w.k;
-      const long long base = w.base(), left = d.count - base;
+      const long long base = w.base() + (threadIdx.x >> 5) * kAdamwChunk, left = d.count - base;
       if (left >= kAdamwChunk) {
         switch (d.grad_type * 2 + d.vec) {
           case 0: adamw32_chunk<GS_TYPE_F32, false>(d, base, a, h, s); break;
@@ -584,30 +607,50 @@ __device__ __forceinline__ void cp_async16(void* dst, const void* src) {
 
 // A chunk on its way: what the copies do not carry.
 struct Adamw8Chunk {
-  long long base;
+  long long tile;  // first element of the CTA's tile
   int k;
-  bool piped;     // copied to shared memory
-  unsigned act;   // flags of the lane's elements
+  int kind;       // copied to shared memory, with no / some / all rows active; or kDirect
+  unsigned act;   // flags of the lane's elements (some)
   unsigned exps;  // exponent byte of mu (lanes 0, 1) or nu (2, 3) of block lane & 1
 };
+constexpr int kNone = 0, kSome = 1, kAll = 2, kDirect = 3;
+
+// Rows of the warp's chunk: none, some or all active, from one flag a lane and row.
+__device__ __forceinline__ int chunk_rows(const AdamwDesc& d, const RowPlace& at, int lane) {
+  const unsigned rows = RowPlace::rows(d, at.rest + kAdamwChunk - 1) + 1;
+  bool all = true, any = false;
+  for (unsigned r = lane; r < rows; r += 32) {
+    const bool f = at.flags[r] != 0;
+    all &= f;
+    any |= f;
+  }
+  return __all_sync(0xffffffffu, all) ? kAll : (__any_sync(0xffffffffu, any) ? kSome : kNone);
+}
 
 __device__ __forceinline__ void adamw8_issue(const AdamwDesc& d, Adamw8Chunk& c, Adamw8Stage& st, int lane) {
-  c.piped = d.vec && d.count - c.base >= kAdamwChunk;
-  if (c.piped) {
-    const char* p = reinterpret_cast<const char*>(d.param + c.base) + 16 * lane;
-    cp_async16(reinterpret_cast<char*>(st.p) + 16 * lane, p);
-    cp_async16(reinterpret_cast<char*>(st.p) + 16 * lane + 512, p + 512);
-    const char* g = static_cast<const char*>(d.grad) + (c.base << (d.grad_type == GS_TYPE_F32 ? 2 : 1)) + 16 * lane;
+  const int chunk = (threadIdx.x >> 5) * kAdamwChunk;
+  c.kind = kDirect;
+  c.act = 0u;
+  if (d.vec && d.count - c.tile >= chunk + kAdamwChunk) {
+    const bool wide = d.grad_type == GS_TYPE_F32;
+    const char* g = static_cast<const char*>(d.grad) + (c.tile << (wide ? 2 : 1)) +
+                    (unsigned)((chunk << (wide ? 2 : 1)) + 16 * lane);
     cp_async16(reinterpret_cast<char*>(st.g) + 16 * lane, g);
-    if (d.grad_type == GS_TYPE_F32) cp_async16(reinterpret_cast<char*>(st.g) + 16 * lane + 512, g + 512);
-    const uint8_t* m = static_cast<const uint8_t*>(lane < 16 ? d.mu : d.nu) + c.base + 16 * (lane & 15);
-    cp_async16((lane < 16 ? st.mu : st.nu) + 16 * (lane & 15), m);
-    c.exps = lane < 4 ? (lane < 2 ? d.mu_exp : d.nu_exp)[c.base / kAdamwBlock + (lane & 1)] : 0u;
-    c.act = 0xFFFFFFFFu;
+    if (wide) cp_async16(reinterpret_cast<char*>(st.g) + 16 * lane + 512, g + 512);
+    const uint8_t* m = static_cast<const uint8_t*>(lane < 16 ? d.mu : d.nu) + c.tile + (unsigned)(chunk + 16 * (lane & 15));
+    cp_async16(st.mu + 16 * lane, m);  // nu's codes follow mu's
+    if (lane < 4) c.exps = ((lane < 2 ? d.mu_exp : d.nu_exp) + c.tile / kAdamwBlock)[(unsigned)(chunk / kAdamwBlock + (lane & 1))];
+    c.kind = kAll;
     if (d.active) {
       RowPlace rows;
-      rows.start(d, (unsigned long long)c.base);
-      c.act = active_bits<true, kAdamwUnroll>(d, rows, 0, lane);
+      rows.start(d, (unsigned long long)(c.tile + chunk));
+      c.kind = chunk_rows(d, rows, lane);
+      if (c.kind == kSome) c.act = active_bits<true, kAdamwUnroll>(d, rows, 0, lane);
+    }
+    if (c.kind != kNone || d.copy) {
+      const char* p = reinterpret_cast<const char*>(d.param + c.tile) + (unsigned)(4 * chunk + 16 * lane);
+      cp_async16(reinterpret_cast<char*>(st.p) + 16 * lane, p);
+      cp_async16(reinterpret_cast<char*>(st.p) + 16 * lane + 512, p + 512);
     }
   }
   asm volatile("cp.async.commit_group;" ::: "memory");
@@ -616,13 +659,14 @@ __device__ __forceinline__ void adamw8_issue(const AdamwDesc& d, Adamw8Chunk& c,
 __device__ __forceinline__ void adamw8_chunk(const AdamwDesc& d, const Adamw8Chunk& c, const Adamw8Stage& st,
                                              const AdamwParams& a, const AdamwStep& h, float s, unsigned key, int lane) {
   constexpr int U = kAdamwUnroll;
-  const unsigned blk0 = (unsigned)(c.base / kAdamwBlock);
-  float* const param = d.param + c.base;
+  const unsigned off = (threadIdx.x >> 5) * kAdamwChunk + 4 * lane;
+  const unsigned blk0 = (unsigned)(c.tile / kAdamwBlock) + (threadIdx.x >> 5) * U;
+  float* const param = d.param + c.tile;
+  unsigned exps = c.exps;
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     const unsigned i = u * kAdamwBlock + 4 * lane;
-    float p[4], g[4], m[4], v[4], fresh[4];
-    load4<true>(st.p, i, p);
+    float g[4], m[4], v[4];
     if (d.grad_type == GS_TYPE_F32) {
       load4<true>(reinterpret_cast<const float*>(st.g), i, g);
     } else {
@@ -633,36 +677,43 @@ __device__ __forceinline__ void adamw8_chunk(const AdamwDesc& d, const Adamw8Chu
         g[q] = d.grad_type == GS_TYPE_BF16 ? __uint_as_float(x[q])
                                            : __half2float(__ushort_as_half((unsigned short)(x[q] >> 16)));
     }
-    unsigned cm = load_codes<true>(st.mu, i), cv = load_codes<true>(st.nu, i);
     int fm = (int)__shfl_sync(0xffffffffu, c.exps, u), fv = (int)__shfl_sync(0xffffffffu, c.exps, 2 + u);
+    if (c.kind == kNone && !d.copy && fm == 0 && fv == 0) {
+      // zero moments of rows that are not active: with a zero gradient nothing changes
+      const unsigned any = (__float_as_uint(g[0]) | __float_as_uint(g[1]) | __float_as_uint(g[2]) |
+                            __float_as_uint(g[3])) << 1;
+      if (__all_sync(0xffffffffu, any == 0u)) continue;
+    }
+    unsigned cm = load_codes<true>(st.mu, i), cv = load_codes<true>(st.nu, i);
     decayed4<true>(cm, fm, a.b1, m);
     decayed4<false>(cv, fv, a.b2, v);
-    float top_m = 0.f, top_v = 0.f;
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
       const float gq = g[q] * s;
       m[q] = add_rn(m[q], mul_rn(gq, a.omb1));
       v[q] = add_rn(v[q], mul_rn(mul_rn(gq, gq), a.omb2));
-      fresh[q] = adamw_param(p[q], m[q], v[q], h, a.eps);
-      top_m = max_abs(top_m, m[q]);
-      top_v = max_abs(top_v, v[q]);
     }
-    const unsigned act = (c.act >> (4 * u)) & 15u;
-    if (!__all_sync(0xffffffffu, act == 15u)) {
+    if (c.kind != kNone || d.copy) {
+      float p[4], fresh[4];
+      load4<true>(st.p, i, p);
+      adamw_param4(p, m, v, h, a, fresh);
+      if (c.kind != kAll) {
 #pragma unroll
-      for (int q = 0; q < 4; ++q)
-        if (!((act >> q) & 1u)) fresh[q] = p[q];
+        for (int q = 0; q < 4; ++q)
+          if (!((c.act >> (4 * u + q)) & 1u)) fresh[q] = p[q];
+      }
+      if (c.kind != kNone) store4<true>(param, off + u * kAdamwBlock, fresh);
+      if (d.copy)
+        store_copy4<true>(static_cast<char*>(d.copy) + c.tile * 2, off + u * kAdamwBlock, d.copy_type, fresh);
     }
-    store4<true>(param, i, fresh);
-    if (d.copy) store_copy4<true>(static_cast<char*>(d.copy) + c.base * 2, i, d.copy_type, fresh);
-    encode_block<true>(m, v, top_m, top_v, key, blk0 + u, lane, cm, cv, fm, fv);
-    store_codes<true>(static_cast<uint8_t*>(d.mu) + c.base, i, cm);
-    store_codes<true>(static_cast<uint8_t*>(d.nu) + c.base, i, cv);
-    if (lane == 0) {
-      (d.mu_exp + c.base / kAdamwBlock)[u] = (uint8_t)fm;
-      (d.nu_exp + c.base / kAdamwBlock)[u] = (uint8_t)fv;
-    }
+    encode_block<true>(m, v, key, blk0 + u, lane, cm, cv, fm, fv);
+    store_codes<true>(static_cast<uint8_t*>(d.mu) + c.tile, off + u * kAdamwBlock, cm);
+    store_codes<true>(static_cast<uint8_t*>(d.nu) + c.tile, off + u * kAdamwBlock, cv);
+    if (lane == u) exps = fm;
+    if (lane == 2 + u) exps = fv;
   }
+  if (lane < 4)
+    ((lane < 2 ? d.mu_exp : d.nu_exp) + c.tile / kAdamwBlock)[(threadIdx.x >> 5) * U + (lane & 1)] = (uint8_t)exps;
 }
 
 template <int N>
@@ -680,13 +731,13 @@ k_adamw8(const __grid_constant__ AdamwTable<N> tab, const __grid_constant__ Adam
     const unsigned key = mix32(a.seed + kGolden * (unsigned)c);
     unsigned tkey = 0u;
     TileWalk<N> w(tab);
-    Adamw8Chunk now, next;
+    Adamw8Chunk now = {}, next = {};
     Adamw8Stage* st = stages[threadIdx.x >> 5];
     int at = 0, last = -1;
     bool more = w.valid();
     if (more) {
       now.k = w.k;
-      now.base = w.base();
+      now.tile = w.base();
       adamw8_issue(tab.t[now.k], now, st[0], lane);
     }
     while (more) {
@@ -694,7 +745,7 @@ k_adamw8(const __grid_constant__ AdamwTable<N> tab, const __grid_constant__ Adam
       more = w.valid();
       if (more) {
         next.k = w.k;
-        next.base = w.base();
+        next.tile = w.base();
         adamw8_issue(tab.t[next.k], next, st[at ^ 1], lane);
         asm volatile("cp.async.wait_group 1;" ::: "memory");
       } else {
@@ -707,12 +758,12 @@ k_adamw8(const __grid_constant__ AdamwTable<N> tab, const __grid_constant__ Adam
         tkey = mix32(key + kGolden * (unsigned)(tab.index0 + now.k));
         last = now.k;
       }
-      if (now.piped) {
+      if (now.kind != kDirect) {
         adamw8_chunk(d, now, st[at], a, h, s, tkey, lane);
       } else {
-        const long long left = d.count - now.base;
+        const long long base = now.tile + (threadIdx.x >> 5) * kAdamwChunk, left = d.count - base;
         for (int e = 0; e < kAdamwChunk && e < left; e += kAdamwBlock)
-          adamw_rest<8>(d, now.base + e, (int)(left - e < kAdamwBlock ? left - e : kAdamwBlock), a, h, s, tkey);
+          adamw_rest<8>(d, base + e, (int)(left - e < kAdamwBlock ? left - e : kAdamwBlock), a, h, s, tkey);
       }
       __syncwarp();  // the stage has been read before it is copied into again
       now = next;
@@ -772,6 +823,7 @@ void launch_adamw(const GsAdamwTensor* tensors, int n, const GsAdamwConfig& cfg,
   a.ln_b1 = (float)std::log(cfg.b1);
   a.ln_b2 = (float)std::log(cfg.b2);
   a.seed = cfg.seed;
+  a.fine_root = a.eps < 0x1p-39f;
   a.scale = scale;
   a.state = state;
   int at = 0;
