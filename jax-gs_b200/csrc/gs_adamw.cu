@@ -50,7 +50,7 @@ static_assert(kAdamwBlock == 128, "a warp holds a block, four elements a lane");
 #define GS_ADAMW_CTAS 3
 #endif
 #ifndef GS_ADAMW8_CTAS
-#define GS_ADAMW8_CTAS 4
+#define GS_ADAMW8_CTAS 5
 #endif
 
 // One tensor as the kernels see it.
@@ -171,6 +171,15 @@ __device__ __forceinline__ float max_abs4(const float x[4]) {
   return r;
 }
 
+__device__ __forceinline__ float max_abs8(const float x[8]) {
+  float r;
+  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(x[0]), "f"(x[1]), "f"(x[2]));
+  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(r), "f"(x[3]), "f"(x[4]));
+  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(r), "f"(x[5]), "f"(x[6]));
+  asm("max.NaN.abs.f32 %0, %1, %2, %2;" : "=f"(r) : "f"(r), "f"(x[7]));
+  return r;
+}
+
 // Element q of a lane in a block: four consecutive elements a lane (16-byte
 // accesses), or, where a pointer is not aligned for that, every 32nd.
 template <bool VEC>
@@ -251,26 +260,6 @@ __device__ __forceinline__ void store_copy4(void* p, unsigned i, int type, const
   }
 }
 
-// Four codes, one to a byte.
-template <bool VEC>
-__device__ __forceinline__ unsigned load_codes(const uint8_t* c, unsigned i) {
-  if (VEC) return *reinterpret_cast<const unsigned*>(c + i);
-  unsigned w = 0u;
-#pragma unroll
-  for (int q = 0; q < 4; ++q) w |= (unsigned)c[i + 32 * q] << (8 * q);
-  return w;
-}
-
-template <bool VEC>
-__device__ __forceinline__ void store_codes(uint8_t* c, unsigned i, unsigned w) {
-  if (VEC) {
-    *reinterpret_cast<unsigned*>(c + i) = w;
-  } else {
-#pragma unroll
-    for (int q = 0; q < 4; ++q) c[i + 32 * q] = (uint8_t)(w >> (8 * q));
-  }
-}
-
 // Place of an element in the rows of an active mask: row and rest. Divisions
 // by the width are multiplications with its rounded-up reciprocal, exact
 // because the numerator times the reciprocal's excess (below the width, at
@@ -290,71 +279,97 @@ struct RowPlace {
   }
 };
 
-// Flags of a lane's elements in U blocks that start `off` elements on, one bit each.
-template <bool VEC, int U>
-__device__ __forceinline__ unsigned active_bits(const AdamwDesc& d, const RowPlace& at, unsigned off, int lane) {
-  unsigned act = 0u;
-#pragma unroll
-  for (int u = 0; u < U; ++u) {
-    if (VEC && d.width >= 4) {  // at most two rows in four elements
-      const unsigned x = at.rest + off + u * kAdamwBlock + 4 * lane;
-      const unsigned r = at.rows(d, x);
-      const unsigned left = (r + 1) * d.width - x;  // elements up to the next row
-      const unsigned head = left >= 4 ? 15u : (1u << left) - 1u;
-      unsigned bits = at.flags[r] != 0 ? head : 0u;
-      if (left < 4 && at.flags[r + 1] != 0) bits |= 15u & ~head;
-      act |= bits << (4 * u);
-    } else {
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const unsigned r = at.rows(d, at.rest + off + u * kAdamwBlock + block_element<VEC>(lane, q));
-        act |= (at.flags[r] != 0 ? 1u : 0u) << (4 * u + q);
-      }
-    }
+// Flags of a lane's four elements from `off` elements on, one bit each.
+template <bool VEC>
+__device__ __forceinline__ unsigned active4(const AdamwDesc& d, const RowPlace& at, unsigned off) {
+  if (VEC && d.width >= 4) {  // at most two rows in four elements
+    const unsigned x = at.rest + off;
+    const unsigned r = RowPlace::rows(d, x);
+    const unsigned left = (r + 1) * d.width - x;  // elements up to the next row
+    const unsigned head = left >= 4 ? 15u : (1u << left) - 1u;
+    unsigned bits = at.flags[r] != 0 ? head : 0u;
+    if (left < 4 && at.flags[r + 1] != 0) bits |= 15u & ~head;
+    return bits;
   }
-  return act;
+  unsigned bits = 0u;
+#pragma unroll
+  for (int q = 0; q < 4; ++q)
+    bits |= (at.flags[RowPlace::rows(d, at.rest + off + (VEC ? q : 32 * q))] != 0 ? 1u : 0u) << q;
+  return bits;
 }
 
-// b times the four moments that a word of codes and an exponent byte stand
-// for. Where the value of every code is a normal float (F >= 18 or 34) and b
-// 2^(F - 127) 2^112 or 2^96 one too, b is folded into the scale: the same
-// single rounding of the same product.
+// b times the four moments that a word of codes stands for, k = b 2^(F - 127)
+// 2^112 or 2^96: with b folded into the scale, the same single rounding of the
+// same product as long as the code's value is exact and k a normal float,
+// F <= 142 (mu) and 11 <= F <= 158 (nu).
 template <bool SIGNED>
-__device__ __forceinline__ void decayed4(unsigned w, int field, float b, float x[4]) {
-  constexpr int kLow = SIGNED ? 18 : 34, kShift = SIGNED ? 15 : 31;
-  if (field >= kLow && field <= 127 + kShift) {
-    const float k = __int_as_float((field - kShift + 127) << 23) * b;
+__device__ __forceinline__ void decayed4(unsigned w, float k, float x[4]) {
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      unsigned y;
-      if (SIGNED) y = (unsigned)((int)__byte_perm(w, 0u, 0x0444 | (q << 12)) >> 4) & 0x87F00000u;
-      else y = (q < 3 ? w << (20 - 8 * q) : w >> 4) & 0x0FF00000u;
-      x[q] = mul_rn(__uint_as_float(y), k);
-    }
-  } else {
-    const float up = field == 255 ? NAN : pow2_biased(field);
-#pragma unroll
-    for (int q = 0; q < 4; ++q) x[q] = mul_rn(decode8<SIGNED>((w >> (8 * q)) & 255u, up), b);
+  for (int q = 0; q < 4; ++q) {
+    unsigned y;
+    if (SIGNED) y = (unsigned)((int)__byte_perm(w, 0u, 0x0444 | (q << 12)) >> 4) & 0x87F00000u;
+    else y = (q < 3 ? w << (20 - 8 * q) : w >> 4) & 0x0FF00000u;
+    x[q] = mul_rn(__uint_as_float(y), k);
   }
+}
+__device__ __forceinline__ bool foldable(int fm, int fv) {
+  return fm <= 142 && (unsigned)(fv - 11) <= 147u;
+}
+template <bool SIGNED>
+__device__ __forceinline__ float folded(int field, float b) {
+  return __int_as_float((field + (SIGNED ? 112 : 96)) << 23) * b;
+}
+
+// The same for any block, in steps.
+template <bool SIGNED>
+__device__ __noinline__ float4 decayed4_any(unsigned w, int field, float b) {
+  const float up = field == 255 ? NAN : pow2_biased(field);
+  float x[4];
+#pragma unroll
+  for (int q = 0; q < 4; ++q) x[q] = mul_rn(decode8<SIGNED>((w >> (8 * q)) & 255u, up), b);
+  return make_float4(x[0], x[1], x[2], x[3]);
 }
 
 // encode8 of four values that `scale` takes to their block's format, one code
-// a byte. No code exceeds the largest: F leaves the largest magnitude at most
-// at the top code, and noise is less than the next code away.
+// a byte, with 16 bits of r as noise: (bits >> 4) + noise has the code in its
+// third byte. No code exceeds the largest: F leaves the largest magnitude at
+// most at the top code, and noise is less than the next code away.
 template <bool SIGNED>
-__device__ __forceinline__ unsigned encode4(const float x[4], float scale, const unsigned noise[4]) {
-  unsigned c[4];
+__device__ __forceinline__ unsigned encode4(const float x[4], float scale, const unsigned r[4]) {
+  unsigned t[4];
 #pragma unroll
-  for (int q = 0; q < 4; ++q) {
-    unsigned t = __float_as_uint(x[q] * scale) + noise[q];
-    if (SIGNED) {
-      c[q] = ((t << 4) & 0x7FFFFFFFu) | (t & 0x80000000u);
-    } else {
-      if (x[q] > 0.f) t = max(t, 1u << 20);
-      c[q] = t << 4;
-    }
+  for (int q = 0; q < 4; ++q)
+    t[q] = (__float_as_uint((SIGNED ? fabsf(x[q]) : x[q]) * scale) >> 4) + (SIGNED ? r[q] & 0xFFFFu : r[q] >> 16);
+  unsigned w = __byte_perm(__byte_perm(t[0], t[1], 0x0062), __byte_perm(t[2], t[3], 0x0062), 0x5410);
+  if (SIGNED) {
+    const unsigned lo = __byte_perm(__float_as_uint(x[0]), __float_as_uint(x[1]), 0x0073);
+    const unsigned hi = __byte_perm(__float_as_uint(x[2]), __float_as_uint(x[3]), 0x0073);
+    w |= __byte_perm(lo, hi, 0x5410) & 0x80808080u;
+  } else if ((w - 0x01010101u) & ~w & 0x80808080u) {  // a code is 0: not if its value is above
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      if (x[q] > 0.f && ((w >> (8 * q)) & 255u) == 0u) w |= 1u << (8 * q);
   }
-  return __byte_perm(__byte_perm(c[0], c[1], 0x0073), __byte_perm(c[2], c[3], 0x0073), 0x5410);
+  return w;
+}
+
+// Scales of a block's new moments, 2^(127 - F) 2^-112 and 2^-96, powers of two
+// as long as those are normal floats; beyond, the values are scaled in two steps.
+template <int K>
+__device__ __forceinline__ void block_scales(float (&m)[K], float (&v)[K], int fm, int fv, float& sm, float& sv) {
+  sm = __int_as_float((142 - fm) << 23);
+  sv = __int_as_float((158 - fv) << 23);
+  if (fm > 141 || fv > 157) {
+    const float dm = pow2_biased(max(254 - fm, 0)), dv = pow2_biased(max(254 - fv, 0));
+#pragma unroll
+    for (int q = 0; q < K; ++q) {
+      m[q] = fm == 255 ? 0.f : m[q] * dm;
+      // a v > 0 stays above 0
+      v[q] = fv == 255 ? 0.f : (v[q] > 0.f ? fmaxf(v[q] * dv, __int_as_float(1)) : 0.f);
+    }
+    sm = 0x1p-112f;
+    sv = 0x1p-96f;
+  }
 }
 
 // Whole blocks with 32-bit moments from element `base` by one warp, all loads
@@ -382,7 +397,9 @@ __device__ __forceinline__ void adamw32_chunk(const AdamwDesc& d, long long base
   if (d.active) {
     RowPlace rows;
     rows.start(d, (unsigned long long)base);
-    act = active_bits<VEC, U>(d, rows, 0, lane);
+    act = 0u;
+#pragma unroll
+    for (int u = 0; u < U; ++u) act |= active4<VEC>(d, rows, u * kAdamwBlock + block_element<VEC>(lane, 0)) << (4 * u);
   }
 #pragma unroll
   for (int u = 0; u < U; ++u) {
@@ -405,38 +422,6 @@ __device__ __forceinline__ void adamw32_chunk(const AdamwDesc& d, long long base
     if (differ4(m1, m[u])) store4<VEC>(mu, i, m1);
     if (differ4(v1, v[u])) store4<VEC>(nu, i, v1);
   }
-}
-
-// The new moments of a block as codes and exponent bytes (fm, fv out). The
-// scales are powers of two, 2^(127 - F) 2^-112 and 2^-96, as long as those are
-// normal floats; beyond, in two steps.
-template <bool VEC>
-__device__ __forceinline__ void encode_block(float m[4], float v[4], unsigned key, unsigned blk, int lane,
-                                             unsigned& cm, unsigned& cv, int& fm, int& fv) {
-  fm = block_field(__reduce_max_sync(0xffffffffu, __float_as_uint(max_abs4(m))));
-  fv = block_field(__reduce_max_sync(0xffffffffu, __float_as_uint(max_abs4(v))));
-  float sm = __int_as_float((142 - fm) << 23), sv = __int_as_float((158 - fv) << 23);
-  if (fm > 141 || fv > 157) {
-    const float dm = pow2_biased(max(254 - fm, 0)), dv = pow2_biased(max(254 - fv, 0));
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      m[q] = fm == 255 ? 0.f : m[q] * dm;
-      // a v > 0 stays above 0
-      v[q] = fv == 255 ? 0.f : (v[q] > 0.f ? fmaxf(v[q] * dv, __int_as_float(1)) : 0.f);
-    }
-    sm = 0x1p-112f;
-    sv = 0x1p-96f;
-  }
-  const unsigned bkey = mix32(key ^ blk) + kGolden * (unsigned)block_element<VEC>(lane, 0);
-  unsigned lo[4], hi[4];
-#pragma unroll
-  for (int q = 0; q < 4; ++q) {
-    const unsigned r = mix32(bkey + kGolden * (unsigned)block_element<VEC>(0, q));
-    lo[q] = (r << 4) & 0xFFFF0u;
-    hi[q] = (r >> 12) & 0xFFFF0u;
-  }
-  cm = encode4<true>(m, sm, lo);
-  cv = encode4<false>(v, sv, hi);
 }
 
 // Up to one block by one warp, `rem` elements of it in range, element by
@@ -469,8 +454,9 @@ __device__ __forceinline__ void adamw_rest(const AdamwDesc& d, long long base, i
     if (!d.active || rows.flags[RowPlace::rows(d, rows.rest + e)] != 0) act |= 1u << q;
   }
   if (BITS == 8) {
-    decayed4<true>(cm, d.mu_exp[blk], a.b1, m);
-    decayed4<false>(cv, d.nu_exp[blk], a.b2, v);
+    const float4 x = decayed4_any<true>(cm, d.mu_exp[blk], a.b1), y = decayed4_any<false>(cv, d.nu_exp[blk], a.b2);
+    m[0] = x.x; m[1] = x.y; m[2] = x.z; m[3] = x.w;
+    v[0] = y.x; v[1] = y.y; v[2] = y.z; v[3] = y.w;
   }
   float fresh[4];
 #pragma unroll
@@ -492,8 +478,16 @@ __device__ __forceinline__ void adamw_rest(const AdamwDesc& d, long long base, i
     }
   }
   if (BITS == 32) return;
-  int fm, fv;
-  encode_block<false>(m, v, key, (unsigned)blk, lane, cm, cv, fm, fv);
+  const int fm = block_field(__reduce_max_sync(0xffffffffu, __float_as_uint(max_abs4(m))));
+  const int fv = block_field(__reduce_max_sync(0xffffffffu, __float_as_uint(max_abs4(v))));
+  const unsigned bkey = mix32(key ^ (unsigned)blk);
+  unsigned r[4];
+#pragma unroll
+  for (int q = 0; q < 4; ++q) r[q] = mix32(bkey + kGolden * (unsigned)(lane + 32 * q));
+  float sm, sv;
+  block_scales(m, v, fm, fv, sm, sv);
+  cm = encode4<true>(m, sm, r);
+  cv = encode4<false>(v, sv, r);
 #pragma unroll
   for (int q = 0; q < 4; ++q) {
     const int e = lane + 32 * q;
@@ -590,14 +584,22 @@ k_adamw32(const __grid_constant__ AdamwTable<N> tab, const __grid_constant__ Ada
   if (a.advance) adamw_advance(a, c, go);
 }
 
-// 8-bit moments. The step costs some 70 instructions an element, about what
-// the SMs can issue in the time that its bytes take, so no warp may wait for
-// memory: each copies its next chunk into shared memory (cp.async, 16 bytes
-// a lane) before it works on the current one.
+// 8-bit moments. The step's instructions take the SMs about as long as its
+// bytes take the memory, so
+//  - no warp waits for memory: each copies its next chunk into shared memory
+//    (cp.async, 16 bytes a lane) before it works on the current one;
+//  - half a warp holds a block, eight elements a lane in two groups of four,
+//    so that what is done once a block is done for two blocks at a time;
+//  - what differs between tensors (gradient type) and chunks (rows that are
+//    not active) is decided once a chunk, not once an element.
+constexpr int kChunk8 = 4 * kAdamwBlock;
+constexpr int kWarps8 = 4;
+static_assert(kChunk8 * kWarps8 == kAdamwTile, "both kernels share the tables' tiles");
+
 struct __align__(16) Adamw8Stage {
-  float p[kAdamwChunk];
-  unsigned g[kAdamwChunk];
-  uint8_t mu[kAdamwChunk], nu[kAdamwChunk];
+  float p[kChunk8];
+  unsigned g[kChunk8];
+  uint8_t mu[kChunk8], nu[kChunk8];
 };
 
 __device__ __forceinline__ void cp_async16(void* dst, const void* src) {
@@ -610,14 +612,20 @@ struct Adamw8Chunk {
   long long tile;  // first element of the CTA's tile
   int k;
   int kind;       // copied to shared memory, with no / some / all rows active; or kDirect
-  unsigned act;   // flags of the lane's elements (some)
-  unsigned exps;  // exponent byte of mu (lanes 0, 1) or nu (2, 3) of block lane & 1
+  unsigned act;   // flags of the lane's elements, group by group (some)
+  unsigned exps;  // exponent byte of mu (lanes 0 .. 3) or nu (4 .. 7) of block lane & 3
 };
 constexpr int kNone = 0, kSome = 1, kAll = 2, kDirect = 3;
 
+// Place in the chunk of group (j, i) of a lane: block 2 j + lane / 16, then
+// elements 64 i + 4 (lane % 16) and on.
+__device__ __forceinline__ int group8(int j, int i, int lane) {
+  return 256 * j + 128 * (lane >> 4) + 64 * i + 4 * (lane & 15);
+}
+
 // Rows of the warp's chunk: none, some or all active, from one flag a lane and row.
 __device__ __forceinline__ int chunk_rows(const AdamwDesc& d, const RowPlace& at, int lane) {
-  const unsigned rows = RowPlace::rows(d, at.rest + kAdamwChunk - 1) + 1;
+  const unsigned rows = RowPlace::rows(d, at.rest + kChunk8 - 1) + 1;
   bool all = true, any = false;
   for (unsigned r = lane; r < rows; r += 32) {
     const bool f = at.flags[r] != 0;
@@ -628,99 +636,165 @@ __device__ __forceinline__ int chunk_rows(const AdamwDesc& d, const RowPlace& at
 }
 
 __device__ __forceinline__ void adamw8_issue(const AdamwDesc& d, Adamw8Chunk& c, Adamw8Stage& st, int lane) {
-  const int chunk = (threadIdx.x >> 5) * kAdamwChunk;
+  const int chunk = (threadIdx.x >> 5) * kChunk8;
   c.kind = kDirect;
-  c.act = 0u;
-  if (d.vec && d.count - c.tile >= chunk + kAdamwChunk) {
-    const bool wide = d.grad_type == GS_TYPE_F32;
-    const char* g = static_cast<const char*>(d.grad) + (c.tile << (wide ? 2 : 1)) +
-                    (unsigned)((chunk << (wide ? 2 : 1)) + 16 * lane);
-    cp_async16(reinterpret_cast<char*>(st.g) + 16 * lane, g);
-    if (wide) cp_async16(reinterpret_cast<char*>(st.g) + 16 * lane + 512, g + 512);
-    const uint8_t* m = static_cast<const uint8_t*>(lane < 16 ? d.mu : d.nu) + c.tile + (unsigned)(chunk + 16 * (lane & 15));
-    cp_async16(st.mu + 16 * lane, m);  // nu's codes follow mu's
-    if (lane < 4) c.exps = ((lane < 2 ? d.mu_exp : d.nu_exp) + c.tile / kAdamwBlock)[(unsigned)(chunk / kAdamwBlock + (lane & 1))];
+  if (d.vec && d.count - c.tile >= chunk + kChunk8) {
+    const int two = d.grad_type == GS_TYPE_F32 ? 2 : 1;
+    const char* g = static_cast<const char*>(d.grad) + (c.tile << two) + (unsigned)((chunk << two) + 16 * lane);
+    char* sg = reinterpret_cast<char*>(st.g) + 16 * lane;
+    cp_async16(sg, g);
+    cp_async16(sg + 512, g + 512);
+    if (two == 2) {
+      cp_async16(sg + 1024, g + 1024);
+      cp_async16(sg + 1536, g + 1536);
+    }
+    cp_async16(st.mu + 16 * lane, static_cast<const uint8_t*>(d.mu) + c.tile + (unsigned)(chunk + 16 * lane));
+    cp_async16(st.nu + 16 * lane, static_cast<const uint8_t*>(d.nu) + c.tile + (unsigned)(chunk + 16 * lane));
+    if (lane < 8)
+      c.exps = ((lane < 4 ? d.mu_exp : d.nu_exp) + c.tile / kAdamwBlock)[(unsigned)(chunk / kAdamwBlock + (lane & 3))];
     c.kind = kAll;
     if (d.active) {
       RowPlace rows;
       rows.start(d, (unsigned long long)(c.tile + chunk));
       c.kind = chunk_rows(d, rows, lane);
-      if (c.kind == kSome) c.act = active_bits<true, kAdamwUnroll>(d, rows, 0, lane);
+      if (c.kind == kSome) {
+        c.act = 0u;
+#pragma unroll
+        for (int n = 0; n < 4; ++n) c.act |= active4<true>(d, rows, group8(n >> 1, n & 1, lane)) << (4 * n);
+      }
     }
     if (c.kind != kNone || d.copy) {
       const char* p = reinterpret_cast<const char*>(d.param + c.tile) + (unsigned)(4 * chunk + 16 * lane);
-      cp_async16(reinterpret_cast<char*>(st.p) + 16 * lane, p);
-      cp_async16(reinterpret_cast<char*>(st.p) + 16 * lane + 512, p + 512);
+      char* sp = reinterpret_cast<char*>(st.p) + 16 * lane;
+#pragma unroll
+      for (int n = 0; n < 4; ++n) cp_async16(sp + 512 * n, p + 512 * n);
     }
   }
   asm volatile("cp.async.commit_group;" ::: "memory");
 }
 
-__device__ __forceinline__ void adamw8_chunk(const AdamwDesc& d, const Adamw8Chunk& c, const Adamw8Stage& st,
-                                             const AdamwParams& a, const AdamwStep& h, float s, unsigned key, int lane) {
-  constexpr int U = kAdamwUnroll;
-  const unsigned off = (threadIdx.x >> 5) * kAdamwChunk + 4 * lane;
-  const unsigned blk0 = (unsigned)(c.tile / kAdamwBlock) + (threadIdx.x >> 5) * U;
-  float* const param = d.param + c.tile;
-  unsigned exps = c.exps;
+template <int GT>
+__device__ __forceinline__ void grads4(const unsigned* st, int e, float g[4]) {
+  if (GT == GS_TYPE_F32) {
+    load4<true>(reinterpret_cast<const float*>(st), e, g);
+  } else {
+    const uint2 w = *reinterpret_cast<const uint2*>(reinterpret_cast<const uint16_t*>(st) + e);
+    const unsigned x[4] = {w.x << 16, w.x & 0xFFFF0000u, w.y << 16, w.y & 0xFFFF0000u};
 #pragma unroll
-  for (int u = 0; u < U; ++u) {
-    const unsigned i = u * kAdamwBlock + 4 * lane;
-    float g[4], m[4], v[4];
-    if (d.grad_type == GS_TYPE_F32) {
-      load4<true>(reinterpret_cast<const float*>(st.g), i, g);
+    for (int q = 0; q < 4; ++q)
+      g[q] = GT == GS_TYPE_BF16 ? __uint_as_float(x[q]) : __half2float(__ushort_as_half((unsigned short)(x[q] >> 16)));
+  }
+}
+
+// Largest of a half warp's exponent bytes, two 16-bit values at a time.
+__device__ __forceinline__ unsigned half_max2(unsigned x) {
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) x = __vmaxu2(x, __shfl_xor_sync(0xffffffffu, x, o));
+  return x;
+}
+
+// Blocks 2 j and 2 j + 1 of a chunk. ALL: every row active, no copy.
+template <int GT, bool ALL>
+__device__ __forceinline__ void adamw8_blocks(const AdamwDesc& d, const Adamw8Chunk& c, const Adamw8Stage& st, int j,
+                                              unsigned& exps, const AdamwParams& a, const AdamwStep& h, float s,
+                                              unsigned key, int lane) {
+  const int src = 2 * j + (lane >> 4);  // the half's block
+  int fm = (int)__shfl_sync(0xffffffffu, c.exps, src), fv = (int)__shfl_sync(0xffffffffu, c.exps, 4 + src);
+  float m[8], v[8];
+  {
+    const unsigned w[4] = {*reinterpret_cast<const unsigned*>(st.mu + group8(j, 0, lane)),
+                           *reinterpret_cast<const unsigned*>(st.mu + group8(j, 1, lane)),
+                           *reinterpret_cast<const unsigned*>(st.nu + group8(j, 0, lane)),
+                           *reinterpret_cast<const unsigned*>(st.nu + group8(j, 1, lane))};
+    if (foldable(fm, fv)) {
+      const float km = folded<true>(fm, a.b1), kv = folded<false>(fv, a.b2);
+      decayed4<true>(w[0], km, m);
+      decayed4<true>(w[1], km, m + 4);
+      decayed4<false>(w[2], kv, v);
+      decayed4<false>(w[3], kv, v + 4);
     } else {
-      const uint2 w = *reinterpret_cast<const uint2*>(reinterpret_cast<const uint16_t*>(st.g) + i);
-      const unsigned x[4] = {w.x << 16, w.x & 0xFFFF0000u, w.y << 16, w.y & 0xFFFF0000u};
 #pragma unroll
-      for (int q = 0; q < 4; ++q)
-        g[q] = d.grad_type == GS_TYPE_BF16 ? __uint_as_float(x[q])
-                                           : __half2float(__ushort_as_half((unsigned short)(x[q] >> 16)));
+      for (int i = 0; i < 2; ++i) {
+        const float4 x = decayed4_any<true>(w[i], fm, a.b1), y = decayed4_any<false>(w[2 + i], fv, a.b2);
+        m[4 * i] = x.x; m[4 * i + 1] = x.y; m[4 * i + 2] = x.z; m[4 * i + 3] = x.w;
+        v[4 * i] = y.x; v[4 * i + 1] = y.y; v[4 * i + 2] = y.z; v[4 * i + 3] = y.w;
+      }
     }
-    int fm = (int)__shfl_sync(0xffffffffu, c.exps, u), fv = (int)__shfl_sync(0xffffffffu, c.exps, 2 + u);
-    if (c.kind == kNone && !d.copy && fm == 0 && fv == 0) {
-      // zero moments of rows that are not active: with a zero gradient nothing changes
-      const unsigned any = (__float_as_uint(g[0]) | __float_as_uint(g[1]) | __float_as_uint(g[2]) |
-                            __float_as_uint(g[3])) << 1;
-      if (__all_sync(0xffffffffu, any == 0u)) continue;
-    }
-    unsigned cm = load_codes<true>(st.mu, i), cv = load_codes<true>(st.nu, i);
-    decayed4<true>(cm, fm, a.b1, m);
-    decayed4<false>(cv, fv, a.b2, v);
+  }
+  const unsigned chunk = (threadIdx.x >> 5) * kChunk8;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int e = group8(j, i, lane);
+    float g[4], p[4], fresh[4];
+    grads4<GT>(st.g, e, g);
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
       const float gq = g[q] * s;
-      m[q] = add_rn(m[q], mul_rn(gq, a.omb1));
-      v[q] = add_rn(v[q], mul_rn(mul_rn(gq, gq), a.omb2));
+      m[4 * i + q] = add_rn(m[4 * i + q], mul_rn(gq, a.omb1));
+      v[4 * i + q] = add_rn(v[4 * i + q], mul_rn(mul_rn(gq, gq), a.omb2));
     }
-    if (c.kind != kNone || d.copy) {
-      float p[4], fresh[4];
-      load4<true>(st.p, i, p);
-      adamw_param4(p, m, v, h, a, fresh);
-      if (c.kind != kAll) {
+    if (ALL || c.kind != kNone || d.copy) {
+      load4<true>(st.p, e, p);
+      adamw_param4(p, m + 4 * i, v + 4 * i, h, a, fresh);
+      if (!ALL && c.kind != kAll) {
 #pragma unroll
         for (int q = 0; q < 4; ++q)
-          if (!((c.act >> (4 * u + q)) & 1u)) fresh[q] = p[q];
+          if (c.kind == kNone || !((c.act >> (8 * j + 4 * i + q)) & 1u)) fresh[q] = p[q];
       }
-      if (c.kind != kNone) store4<true>(param, off + u * kAdamwBlock, fresh);
-      if (d.copy)
-        store_copy4<true>(static_cast<char*>(d.copy) + c.tile * 2, off + u * kAdamwBlock, d.copy_type, fresh);
+      if (ALL || c.kind != kNone) store4<true>(d.param + c.tile, chunk + e, fresh);
+      if (!ALL && d.copy)
+        store_copy4<true>(static_cast<char*>(d.copy) + c.tile * 2, chunk + e, d.copy_type, fresh);
     }
-    encode_block<true>(m, v, key, blk0 + u, lane, cm, cv, fm, fv);
-    store_codes<true>(static_cast<uint8_t*>(d.mu) + c.tile, off + u * kAdamwBlock, cm);
-    store_codes<true>(static_cast<uint8_t*>(d.nu) + c.tile, off + u * kAdamwBlock, cv);
-    if (lane == u) exps = fm;
-    if (lane == 2 + u) exps = fv;
   }
-  if (lane < 4)
-    ((lane < 2 ? d.mu_exp : d.nu_exp) + c.tile / kAdamwBlock)[(threadIdx.x >> 5) * U + (lane & 1)] = (uint8_t)exps;
+  const unsigned top = half_max2((unsigned)block_field(__float_as_uint(max_abs8(m))) |
+                                 (unsigned)block_field(__float_as_uint(max_abs8(v))) << 16);
+  fm = (int)(top & 0xFFFFu);
+  fv = (int)(top >> 16);
+  float sm, sv;
+  block_scales(m, v, fm, fv, sm, sv);
+  const unsigned bkey = mix32(key ^ ((unsigned)(c.tile / kAdamwBlock) + chunk / kAdamwBlock + (unsigned)src)) +
+                        kGolden * (unsigned)(4 * (lane & 15));
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    unsigned r[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) r[q] = mix32(bkey + kGolden * (unsigned)(64 * i + q));
+    const unsigned at = chunk + (unsigned)group8(j, i, lane);
+    *reinterpret_cast<unsigned*>(static_cast<uint8_t*>(d.mu) + c.tile + at) = encode4<true>(m + 4 * i, sm, r);
+    *reinterpret_cast<unsigned*>(static_cast<uint8_t*>(d.nu) + c.tile + at) = encode4<false>(v + 4 * i, sv, r);
+  }
+  // lane b collects the byte of mu of block b, lane 4 + b that of nu
+  const unsigned both = __shfl_sync(0xffffffffu, top, (lane & 1) << 4);
+  if ((lane & 3) >> 1 == j) exps = lane < 4 ? both & 0xFFFFu : both >> 16;
+}
+
+template <int GT, bool ALL>
+__device__ __forceinline__ void adamw8_chunk(const AdamwDesc& d, const Adamw8Chunk& c, const Adamw8Stage& st,
+                                             const AdamwParams& a, const AdamwStep& h, float s, unsigned key, int lane) {
+  unsigned exps = 0u;
+  if (!ALL && c.kind == kNone && !d.copy) {
+    // moments and gradients all zero in rows that are not active: nothing changes
+    unsigned any = lane < 8 ? c.exps : 0u;
+#pragma unroll
+    for (int n = 0; n < 4; ++n) {
+      float g[4];
+      grads4<GT>(st.g, group8(n >> 1, n & 1, lane), g);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) any |= __float_as_uint(g[q]) << 1;
+    }
+    if (__all_sync(0xffffffffu, any == 0u)) return;
+  }
+#pragma unroll
+  for (int j = 0; j < 2; ++j) adamw8_blocks<GT, ALL>(d, c, st, j, exps, a, h, s, key, lane);
+  if (lane < 8)
+    ((lane < 4 ? d.mu_exp : d.nu_exp) + c.tile / kAdamwBlock)[(threadIdx.x >> 5) * 4 + (lane & 3)] = (uint8_t)exps;
 }
 
 template <int N>
-__global__ void __launch_bounds__(32 * kAdamwWarps, GS_ADAMW8_CTAS)
+__global__ void __launch_bounds__(32 * kWarps8, GS_ADAMW8_CTAS)
 k_adamw8(const __grid_constant__ AdamwTable<N> tab, const __grid_constant__ AdamwParams a) {
   GS_PDL_ENTRY_PLAIN();
-  __shared__ Adamw8Stage stages[kAdamwWarps][2];
+  __shared__ Adamw8Stage stages[kWarps8][2];
   const int c = *(volatile int*)a.state;
   const float s = a.scale ? *(volatile const float*)a.scale : 1.f;
   const bool go = fabsf(s) <= 3.402823466e38f;
@@ -759,10 +833,18 @@ k_adamw8(const __grid_constant__ AdamwTable<N> tab, const __grid_constant__ Adam
         last = now.k;
       }
       if (now.kind != kDirect) {
-        adamw8_chunk(d, now, st[at], a, h, s, tkey, lane);
+        const bool all = now.kind == kAll && !d.copy;
+        switch (d.grad_type * 2 + all) {
+          case 0: adamw8_chunk<GS_TYPE_F32, false>(d, now, st[at], a, h, s, tkey, lane); break;
+          case 1: adamw8_chunk<GS_TYPE_F32, true>(d, now, st[at], a, h, s, tkey, lane); break;
+          case 2: adamw8_chunk<GS_TYPE_BF16, false>(d, now, st[at], a, h, s, tkey, lane); break;
+          case 3: adamw8_chunk<GS_TYPE_BF16, true>(d, now, st[at], a, h, s, tkey, lane); break;
+          case 4: adamw8_chunk<GS_TYPE_F16, false>(d, now, st[at], a, h, s, tkey, lane); break;
+          default: adamw8_chunk<GS_TYPE_F16, true>(d, now, st[at], a, h, s, tkey, lane); break;
+        }
       } else {
-        const long long base = now.tile + (threadIdx.x >> 5) * kAdamwChunk, left = d.count - base;
-        for (int e = 0; e < kAdamwChunk && e < left; e += kAdamwBlock)
+        const long long base = now.tile + (threadIdx.x >> 5) * kChunk8, left = d.count - base;
+        for (int e = 0; e < kChunk8 && e < left; e += kAdamwBlock)
           adamw_rest<8>(d, base + e, (int)(left - e < kAdamwBlock ? left - e : kAdamwBlock), a, h, s, tkey);
       }
       __syncwarp();  // the stage has been read before it is copied into again
@@ -807,7 +889,8 @@ static void launch_adamw_class(const GsAdamwTensor* t, int n, int index0, const 
   tab.index0 = index0;
   const int grid = std::max(1, std::min(tiles, device_sms() * (BITS == 8 ? GS_ADAMW8_CTAS : 8)));
   GS_TIMED(BITS == 8 ? "adamw8" : "adamw", st);
-  launch_kernel_plain(BITS == 8 ? k_adamw8<N> : k_adamw32<N>, grid, 32 * kAdamwWarps, 0, st, tab, a);
+  if (BITS == 8) launch_kernel_plain(k_adamw8<N>, grid, 32 * kWarps8, 0, st, tab, a);
+  else launch_kernel_plain(k_adamw32<N>, grid, 32 * kAdamwWarps, 0, st, tab, a);
 }
 
 constexpr int kAdamwSmall = 8, kAdamwMost = 256;
