@@ -46,6 +46,15 @@ constexpr int kAdamwUnroll = 2;  // blocks of a chunk, what a warp takes at a ti
 constexpr int kAdamwChunk = kAdamwBlock * kAdamwUnroll;
 constexpr int kAdamwTile = kAdamwChunk * kAdamwWarps;  // elements a CTA takes at a time
 static_assert(kAdamwBlock == 128, "a warp holds a block, four elements a lane");
+#ifndef GS_DECODE_UNROLL
+#define GS_DECODE_UNROLL 2
+#endif
+#ifndef GS_NORM_VECS
+#define GS_NORM_VECS 4
+#endif
+#ifndef GS_NORM_CTAS
+#define GS_NORM_CTAS 4
+#endif
 #ifndef GS_ADAMW_CTAS
 #define GS_ADAMW_CTAS 3
 #endif
@@ -946,7 +955,7 @@ struct GradTable {
 // A tile is 16 KB of a tensor counted from the 16-byte boundary at or before
 // its first element, 64 bytes a thread in 16-byte loads; only the vectors
 // that hold both the tensor's elements and others are read one by one.
-constexpr int kNormVecs = 4;
+constexpr int kNormVecs = GS_NORM_VECS;
 constexpr int kNormTileBytes = 256 * 16 * kNormVecs;
 
 __host__ __device__ __forceinline__ long long norm_tiles(const void* grad, long long count, int type) {
@@ -955,53 +964,60 @@ __host__ __device__ __forceinline__ long long norm_tiles(const void* grad, long 
 }
 
 template <int GT>
+__device__ __forceinline__ void norm_add(const uint4& w, double acc[4]) {
+  const unsigned b[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    if (GT == GS_TYPE_F32) {
+      const double x = (double)__uint_as_float(b[q]);
+      acc[q] = fma(x, x, acc[q]);
+    } else {
+      float lo, hi;
+      if (GT == GS_TYPE_BF16) {
+        lo = __uint_as_float(b[q] << 16);
+        hi = __uint_as_float(b[q] & 0xFFFF0000u);
+      } else {
+        lo = __half2float(__ushort_as_half((unsigned short)(b[q] & 0xFFFFu)));
+        hi = __half2float(__ushort_as_half((unsigned short)(b[q] >> 16)));
+      }
+      const double x = (double)lo, y = (double)hi;
+      acc[q] = fma(x, x, acc[q]);
+      acc[q] = fma(y, y, acc[q]);
+    }
+  }
+}
+
+template <int GT>
 __device__ __forceinline__ void norm_tile(const GradDesc& d, long long tile, double acc[4]) {
   constexpr int PER = GT == GS_TYPE_F32 ? 4 : 8;  // elements of a vector
   const unsigned shift = (unsigned)((uintptr_t)d.grad & 15) / (16 / PER);
-  const uint4* vecs = reinterpret_cast<const uint4*>((uintptr_t)d.grad & ~(uintptr_t)15);
-  const long long v0 = tile * (256 * kNormVecs) + threadIdx.x;
-  uint4 w[kNormVecs];
+  const long long v0 = tile * (256 * kNormVecs);  // the tile's first vector; its first element is v0 PER - shift
+  const uint4* vecs = reinterpret_cast<const uint4*>((uintptr_t)d.grad & ~(uintptr_t)15) + v0;
+  if (v0 * PER >= shift && (v0 + 256 * kNormVecs) * PER - shift <= d.count) {  // all of it in the tensor
+    uint4 w[kNormVecs];
 #pragma unroll
+    for (int j = 0; j < kNormVecs; ++j) w[j] = __ldg(vecs + threadIdx.x + 256 * j);
+#pragma unroll
+    for (int j = 0; j < kNormVecs; ++j) norm_add<GT>(w[j], acc);
+    return;
+  }
   for (int j = 0; j < kNormVecs; ++j) {
-    const long long e = (v0 + 256 * j) * PER - shift;  // the vector's first element
-    w[j] = make_uint4(0u, 0u, 0u, 0u);
+    const unsigned k = threadIdx.x + 256 * j;
+    const long long e = (v0 + k) * PER - shift;
     if (e >= 0 && e + PER <= d.count) {
-      w[j] = __ldg(vecs + v0 + 256 * j);
+      norm_add<GT>(__ldg(vecs + k), acc);
     } else if (e + PER > 0 && e < d.count) {
       for (int q = 0; q < PER; ++q)
         if (e + q >= 0 && e + q < d.count) {
           const double x = (double)load_as_float(d.grad, e + q, GT);
-          acc[0] += x * x;
+          acc[0] = fma(x, x, acc[0]);
         }
-    }
-  }
-#pragma unroll
-  for (int j = 0; j < kNormVecs; ++j) {
-    const unsigned b[4] = {w[j].x, w[j].y, w[j].z, w[j].w};
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      if (GT == GS_TYPE_F32) {
-        const double x = (double)__uint_as_float(b[q]);
-        acc[q] = fma(x, x, acc[q]);
-      } else {
-        float lo, hi;
-        if (GT == GS_TYPE_BF16) {
-          lo = __uint_as_float(b[q] << 16);
-          hi = __uint_as_float(b[q] & 0xFFFF0000u);
-        } else {
-          lo = __half2float(__ushort_as_half((unsigned short)(b[q] & 0xFFFFu)));
-          hi = __half2float(__ushort_as_half((unsigned short)(b[q] >> 16)));
-        }
-        const double x = (double)lo, y = (double)hi;
-        acc[q] = fma(x, x, acc[q]);
-        acc[q] = fma(y, y, acc[q]);
-      }
     }
   }
 }
 
 template <int N>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(256, GS_NORM_CTAS)
 k_grad_norm(const __grid_constant__ GradTable<N> tab, double* __restrict__ partials, int part0, int parts,
             float max_norm, const float* __restrict__ unscale, GsGradNorm* __restrict__ out) {
   GS_PDL_ENTRY_PLAIN();
@@ -1010,13 +1026,13 @@ k_grad_norm(const __grid_constant__ GradTable<N> tab, double* __restrict__ parti
   double sums[4] = {0.0, 0.0, 0.0, 0.0};
   const int tiles = tab.first[tab.n];
   int k = 0;
+  for (int hi = tab.n; hi - k > 1;) {
+    const int mid = (k + hi) >> 1;
+    if (tab.first[mid] <= (int)blockIdx.x) k = mid;
+    else hi = mid;
+  }
   for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
-    int hi = tab.n;
-    while (hi - k > 1) {
-      const int mid = (k + hi) >> 1;
-      if (tab.first[mid] <= tile) k = mid;
-      else hi = mid;
-    }
+    while (tab.first[k + 1] <= tile) ++k;
     const GradDesc& d = tab.t[k];
     const long long t = tile - tab.first[k];
     if (d.type == GS_TYPE_F32) norm_tile<GS_TYPE_F32>(d, t, sums);
@@ -1107,27 +1123,72 @@ void launch_grad_norm(const GsGradTensor* tensors, int n, float max_norm, const 
 // ---------------------------------------------------------------------------
 // 8-bit moments to and from values, one warp a block. Encoding rounds to
 // nearest (halves up): values that came from codes are kept exactly.
-template <typename T>
-__device__ __forceinline__ T from_float(float x);
-template <>
-__device__ __forceinline__ float from_float<float>(float x) { return x; }
-template <>
-__device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
+__device__ __forceinline__ void store_value(float* p, float x) { *p = x; }
+__device__ __forceinline__ void store_value(__nv_bfloat16* p, float x) { *p = __float2bfloat16_rn(x); }
 
-template <typename T>
+__device__ __forceinline__ void store_values4(float* p, const float x[4]) {
+  *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]);
+}
+__device__ __forceinline__ void store_values4(__nv_bfloat16* p, const float x[4]) {
+  const __nv_bfloat162 a = __floats2bfloat162_rn(x[0], x[1]), b = __floats2bfloat162_rn(x[2], x[3]);
+  *reinterpret_cast<uint2*>(p) = make_uint2(*reinterpret_cast<const unsigned*>(&a), *reinterpret_cast<const unsigned*>(&b));
+}
+
+template <bool SIGNED>
+__device__ __forceinline__ void values4(unsigned w, int field, float x[4]) {
+  if (SIGNED ? field <= 142 : (unsigned)(field - 11) <= 147u) {
+    decayed4<SIGNED>(w, folded<SIGNED>(field, 1.f), x);
+  } else {
+    const float4 y = decayed4_any<SIGNED>(w, field, 1.f);
+    x[0] = y.x; x[1] = y.y; x[2] = y.z; x[3] = y.w;
+  }
+}
+
+// VEC: four codes of each moment a thread and turn, 2 turns in flight; else one.
+template <typename T, bool VEC>
 __global__ void __launch_bounds__(256)
 k_moments8_decode(const uint8_t* __restrict__ mu, const uint8_t* __restrict__ nu, const uint8_t* __restrict__ mu_exp,
                   const uint8_t* __restrict__ nu_exp, long long count, T* __restrict__ mu_out,
                   T* __restrict__ nu_out) {
   GS_PDL_ENTRY_PLAIN();
   const long long stride = (long long)gridDim.x * 256;
-  for (long long i = blockIdx.x * 256ll + threadIdx.x; i < count; i += stride) {
-    const long long blk = i / kAdamwBlock;
-    const int fm = mu_exp[blk], fv = nu_exp[blk];
+  long long i = blockIdx.x * 256ll + threadIdx.x;
+  if (VEC) {
+    constexpr int U = GS_DECODE_UNROLL;
+    const long long n4 = count / 4;
+    for (; i < n4; i += U * stride) {
+      unsigned wm[U], wv[U];
+      int fm[U], fv[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const long long k = i + u * stride;
+        if (k < n4) {
+          wm[u] = reinterpret_cast<const unsigned*>(mu)[k];
+          wv[u] = reinterpret_cast<const unsigned*>(nu)[k];
+          fm[u] = mu_exp[k / (kAdamwBlock / 4)];
+          fv[u] = nu_exp[k / (kAdamwBlock / 4)];
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const long long k = i + u * stride;
+        if (k < n4) {
+          float x[4];
+          values4<true>(wm[u], fm[u], x);
+          store_values4(mu_out + 4 * k, x);
+          values4<false>(wv[u], fv[u], x);
+          store_values4(nu_out + 4 * k, x);
+        }
+      }
+    }
+    i = 4 * n4 + blockIdx.x * 256ll + threadIdx.x;  // the last few
+  }
+  for (; i < count; i += stride) {
+    const int fm = mu_exp[i / kAdamwBlock], fv = nu_exp[i / kAdamwBlock];
     const float m = decode8<true>(mu[i], pow2_biased(min(fm, 254)));
     const float v = decode8<false>(nu[i], pow2_biased(min(fv, 254)));
-    mu_out[i] = from_float<T>(fm == 255 ? NAN : m);
-    nu_out[i] = from_float<T>(fv == 255 ? NAN : v);
+    store_value(mu_out + i, fm == 255 ? NAN : m);
+    store_value(nu_out + i, fv == 255 ? NAN : v);
   }
 }
 
@@ -1168,14 +1229,23 @@ k_moments8_encode(const float* __restrict__ mu, const float* __restrict__ nu, lo
 
 void launch_moments8_decode(const uint8_t* mu, const uint8_t* nu, const uint8_t* mu_exp, const uint8_t* nu_exp,
                             long long count, int type, void* mu_out, void* nu_out, cudaStream_t st) {
-  const int grid = (int)std::min((count + 255) / 256, (long long)device_sms() * 8);
+  const uintptr_t bits = (uintptr_t)mu_out | (uintptr_t)nu_out;
+  const bool vec = (bits & (type == GS_TYPE_F32 ? 15 : 7)) == 0;  // the codes are 4-byte aligned
+  const long long items = vec ? count / 4 + 3 : count;
+  const int grid = (int)std::min((items + 255) / 256, (long long)device_sms() * 8);
   GS_TIMED("moments8_decode", st);
-  if (type == GS_TYPE_F32)
-    launch_kernel_plain(k_moments8_decode<float>, grid, 256, 0, st, mu, nu, mu_exp, nu_exp, count,
-                        static_cast<float*>(mu_out), static_cast<float*>(nu_out));
-  else
-    launch_kernel_plain(k_moments8_decode<__nv_bfloat16>, grid, 256, 0, st, mu, nu, mu_exp, nu_exp, count,
-                        static_cast<__nv_bfloat16*>(mu_out), static_cast<__nv_bfloat16*>(nu_out));
+  auto launch = [&](auto kernel, auto* m, auto* v) {
+    launch_kernel_plain(kernel, grid, 256, 0, st, mu, nu, mu_exp, nu_exp, count, m, v);
+  };
+  if (type == GS_TYPE_F32) {
+    float *m = static_cast<float*>(mu_out), *v = static_cast<float*>(nu_out);
+    if (vec) launch(k_moments8_decode<float, true>, m, v);
+    else launch(k_moments8_decode<float, false>, m, v);
+  } else {
+    __nv_bfloat16 *m = static_cast<__nv_bfloat16*>(mu_out), *v = static_cast<__nv_bfloat16*>(nu_out);
+    if (vec) launch(k_moments8_decode<__nv_bfloat16, true>, m, v);
+    else launch(k_moments8_decode<__nv_bfloat16, false>, m, v);
+  }
 }
 
 void launch_moments8_encode(const float* mu, const float* nu, long long count, uint8_t* mu8, uint8_t* nu8,
