@@ -46,6 +46,9 @@ constexpr int kAdamwUnroll = 2;  // blocks of a chunk, what a warp takes at a ti
 constexpr int kAdamwChunk = kAdamwBlock * kAdamwUnroll;
 constexpr int kAdamwTile = kAdamwChunk * kAdamwWarps;  // elements a CTA takes at a time
 static_assert(kAdamwBlock == 128, "a warp holds a block, four elements a lane");
+#ifndef GS_ADAMW_SMALL
+#define GS_ADAMW_SMALL 32
+#endif
 #ifndef GS_DECODE_UNROLL
 #define GS_DECODE_UNROLL 2
 #endif
@@ -434,93 +437,151 @@ __device__ __forceinline__ void adamw32_chunk(const AdamwDesc& d, long long base
 }
 
 // Up to one block by one warp, `rem` elements of it in range, element by
-// element: the end of a tensor, and, with 8-bit moments, tensors whose
-// pointers are not 16-byte aligned.
+// element: the ends of tensors, few elements in all, and, with 8-bit moments,
+// tensors whose pointers are not 16-byte aligned.
 template <int BITS>
-__device__ __forceinline__ void adamw_rest(const AdamwDesc& d, long long base, int rem, const AdamwParams& a,
-                                           const AdamwStep& h, float s, unsigned key) {
-  const int lane = threadIdx.x & 31;
-  const long long blk = base / kAdamwBlock;
-  RowPlace rows;
-  if (d.active) rows.start(d, (unsigned long long)base);
+struct AdamwBlock {
+  long long base;
+  int rem;
   float p[4], g[4], m[4], v[4];
-  unsigned cm = 0u, cv = 0u, act = 0u;
+  unsigned cm, cv, act;
+  int fm, fv;
+
+  __device__ __forceinline__ void load(const AdamwDesc& d, long long from, int in_range) {
+    const int lane = threadIdx.x & 31;
+    base = from;
+    rem = in_range;
+    RowPlace rows;
+    if (d.active) rows.start(d, (unsigned long long)base);
+    cm = cv = act = 0u;
 #pragma unroll
-  for (int q = 0; q < 4; ++q) {
-    p[q] = g[q] = m[q] = v[q] = 0.f;
-    const int e = lane + 32 * q;
-    const long long i = base + e;
-    if (e >= rem) continue;
-    p[q] = d.param[i];
-    g[q] = load_as_float(d.grad, i, d.grad_type) * s;
+    for (int q = 0; q < 4; ++q) {
+      p[q] = g[q] = m[q] = v[q] = 0.f;
+      const int e = lane + 32 * q;
+      const long long i = base + e;
+      if (e >= rem) continue;
+      p[q] = d.param[i];
+      g[q] = load_as_float(d.grad, i, d.grad_type);
+      if (BITS == 8) {
+        cm |= (unsigned)static_cast<const uint8_t*>(d.mu)[i] << (8 * q);
+        cv |= (unsigned)static_cast<const uint8_t*>(d.nu)[i] << (8 * q);
+      } else {
+        m[q] = static_cast<const float*>(d.mu)[i];
+        v[q] = static_cast<const float*>(d.nu)[i];
+      }
+      if (!d.active || rows.flags[RowPlace::rows(d, rows.rest + e)] != 0) act |= 1u << q;
+    }
     if (BITS == 8) {
-      cm |= (unsigned)static_cast<const uint8_t*>(d.mu)[i] << (8 * q);
-      cv |= (unsigned)static_cast<const uint8_t*>(d.nu)[i] << (8 * q);
-    } else {
-      m[q] = mul_rn(static_cast<const float*>(d.mu)[i], a.b1);
-      v[q] = mul_rn(static_cast<const float*>(d.nu)[i], a.b2);
-    }
-    if (!d.active || rows.flags[RowPlace::rows(d, rows.rest + e)] != 0) act |= 1u << q;
-  }
-  if (BITS == 8) {
-    const float4 x = decayed4_any<true>(cm, d.mu_exp[blk], a.b1), y = decayed4_any<false>(cv, d.nu_exp[blk], a.b2);
-    m[0] = x.x; m[1] = x.y; m[2] = x.z; m[3] = x.w;
-    v[0] = y.x; v[1] = y.y; v[2] = y.z; v[3] = y.w;
-  }
-  float fresh[4];
-#pragma unroll
-  for (int q = 0; q < 4; ++q) {
-    const bool in = lane + 32 * q < rem;  // else zeros, which leave no trace in the block
-    m[q] = in ? add_rn(m[q], mul_rn(g[q], a.omb1)) : 0.f;
-    v[q] = in ? add_rn(v[q], mul_rn(mul_rn(g[q], g[q]), a.omb2)) : 0.f;
-  }
-  adamw_param4(p, m, v, h, a, fresh);
-#pragma unroll
-  for (int q = 0; q < 4; ++q) {
-    const long long i = base + lane + 32 * q;
-    if (lane + 32 * q >= rem) continue;
-    if ((act >> q) & 1u) d.param[i] = p[q] = fresh[q];
-    if (d.copy) store_as(d.copy, i, d.copy_type, p[q]);
-    if (BITS == 32) {
-      static_cast<float*>(d.mu)[i] = m[q];
-      static_cast<float*>(d.nu)[i] = v[q];
+      fm = d.mu_exp[base / kAdamwBlock];
+      fv = d.nu_exp[base / kAdamwBlock];
     }
   }
-  if (BITS == 32) return;
-  const int fm = block_field(__reduce_max_sync(0xffffffffu, __float_as_uint(max_abs4(m))));
-  const int fv = block_field(__reduce_max_sync(0xffffffffu, __float_as_uint(max_abs4(v))));
-  const unsigned bkey = mix32(key ^ (unsigned)blk);
-  unsigned r[4];
+
+  __device__ __forceinline__ void step(const AdamwDesc& d, const AdamwParams& a, const AdamwStep& h, float s,
+                                       unsigned key) {
+    const int lane = threadIdx.x & 31;
+    const long long blk = base / kAdamwBlock;
+    if (BITS == 8) {
+      const float4 x = decayed4_any<true>(cm, fm, a.b1), y = decayed4_any<false>(cv, fv, a.b2);
+      m[0] = x.x; m[1] = x.y; m[2] = x.z; m[3] = x.w;
+      v[0] = y.x; v[1] = y.y; v[2] = y.z; v[3] = y.w;
+    }
+    float fresh[4];
 #pragma unroll
-  for (int q = 0; q < 4; ++q) r[q] = mix32(bkey + kGolden * (unsigned)(lane + 32 * q));
-  float sm, sv;
-  block_scales(m, v, fm, fv, sm, sv);
-  cm = encode4<true>(m, sm, r);
-  cv = encode4<false>(v, sv, r);
+    for (int q = 0; q < 4; ++q) {
+      const bool in = lane + 32 * q < rem;  // else zeros, which leave no trace in the block
+      const float gq = g[q] * s;
+      if (BITS == 32) {
+        m[q] = mul_rn(m[q], a.b1);
+        v[q] = mul_rn(v[q], a.b2);
+      }
+      m[q] = in ? add_rn(m[q], mul_rn(gq, a.omb1)) : 0.f;
+      v[q] = in ? add_rn(v[q], mul_rn(mul_rn(gq, gq), a.omb2)) : 0.f;
+    }
+    adamw_param4(p, m, v, h, a, fresh);
 #pragma unroll
-  for (int q = 0; q < 4; ++q) {
-    const int e = lane + 32 * q;
-    if (e >= rem) continue;
-    static_cast<uint8_t*>(d.mu)[base + e] = (uint8_t)(cm >> (8 * q));
-    static_cast<uint8_t*>(d.nu)[base + e] = (uint8_t)(cv >> (8 * q));
+    for (int q = 0; q < 4; ++q) {
+      const long long i = base + lane + 32 * q;
+      if (lane + 32 * q >= rem) continue;
+      if ((act >> q) & 1u) d.param[i] = p[q] = fresh[q];
+      if (d.copy) store_as(d.copy, i, d.copy_type, p[q]);
+      if (BITS == 32) {
+        static_cast<float*>(d.mu)[i] = m[q];
+        static_cast<float*>(d.nu)[i] = v[q];
+      }
+    }
+    if (BITS == 32) return;
+    fm = block_field(__reduce_max_sync(0xffffffffu, __float_as_uint(max_abs4(m))));
+    fv = block_field(__reduce_max_sync(0xffffffffu, __float_as_uint(max_abs4(v))));
+    const unsigned bkey = mix32(key ^ (unsigned)blk);
+    unsigned r[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) r[q] = mix32(bkey + kGolden * (unsigned)(lane + 32 * q));
+    float sm, sv;
+    block_scales(m, v, fm, fv, sm, sv);
+    cm = encode4<true>(m, sm, r);
+    cv = encode4<false>(v, sv, r);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int e = lane + 32 * q;
+      if (e >= rem) continue;
+      static_cast<uint8_t*>(d.mu)[base + e] = (uint8_t)(cm >> (8 * q));
+      static_cast<uint8_t*>(d.nu)[base + e] = (uint8_t)(cv >> (8 * q));
+    }
+    if (lane == 0) {
+      d.mu_exp[blk] = (uint8_t)fm;
+      d.nu_exp[blk] = (uint8_t)fv;
+    }
   }
-  if (lane == 0) {
-    d.mu_exp[blk] = (uint8_t)fm;
-    d.nu_exp[blk] = (uint8_t)fv;
+};
+
+// The blocks of [base, base + chunk) that are in the tensor, one by one.
+template <int BITS>
+__device__ __forceinline__ void adamw_blocks(const AdamwDesc& d, long long base, int chunk, const AdamwParams& a,
+                                             const AdamwStep& h, float s, unsigned key) {
+  const long long left = d.count - base;
+#pragma unroll 1
+  for (int e = 0; e < chunk && e < left; e += kAdamwBlock) {
+    AdamwBlock<BITS> b;
+    b.load(d, base + e, (int)(left - e < kAdamwBlock ? left - e : kAdamwBlock));
+    b.step(d, a, h, s, key);
   }
 }
 
-// The last CTA to finish (atomic ticket, no waiting) advances the count.
-__device__ __forceinline__ void adamw_advance(const AdamwParams& a, int c, bool go) {
-  __syncthreads();
+// What a step takes from the device: count, scale, bias corrections (1 - b^t
+// as -expm1(t ln b): no cancellation at small t), read by one thread of the
+// CTA. Its ticket is drawn after the read (an acquire) and looked at when the
+// CTA's work is done: the CTA with the last ticket knows that every CTA has
+// read the count, and advances it. Nothing waits for another CTA.
+struct AdamwHead {
+  int c;
+  float s, inv1, inv2;
+  bool go;
+};
+
+__device__ __forceinline__ unsigned adamw_head(const AdamwParams& a, AdamwHead& head) {
+  unsigned ticket = 0u;
   if (threadIdx.x == 0) {
-    __threadfence();
-    const unsigned t = atomicAdd(reinterpret_cast<unsigned*>(a.state + 1), 1u);
-    if (t == gridDim.x - 1) {
-      if (go) a.state[0] = c + 1;
-      else a.state[2] = a.state[2] + 1;
-      a.state[1] = 0;
-    }
+    int c;
+    asm volatile("ld.acquire.gpu.global.s32 %0, [%1];" : "=r"(c) : "l"(a.state) : "memory");
+    const float s = a.scale ? *(volatile const float*)a.scale : 1.f;
+    if (a.advance) ticket = atomicAdd(reinterpret_cast<unsigned*>(a.state + 1), 1u);
+    const float t = (float)c + 1.f;
+    head.c = c;
+    head.s = s;
+    head.go = fabsf(s) <= 3.402823466e38f;
+    head.inv1 = 1.f / -expm1f(t * a.ln_b1);
+    head.inv2 = 1.f / -expm1f(t * a.ln_b2);
+  }
+  __syncthreads();
+  return ticket;
+}
+
+__device__ __forceinline__ void adamw_finish(const AdamwParams& a, const AdamwHead& head, unsigned ticket) {
+  if (threadIdx.x == 0 && a.advance && ticket == gridDim.x - 1) {
+    if (head.go) a.state[0] = head.c + 1;
+    else a.state[2] = a.state[2] + 1;
+    a.state[1] = 0;
   }
 }
 
@@ -548,11 +609,7 @@ struct TileWalk {
   __device__ __forceinline__ long long base() const { return (long long)(tile - tab.first[k]) * kAdamwTile; }
 };
 
-// Step values of a tensor. 1 - b^t as -expm1(t ln b): no cancellation at small t.
-__device__ __forceinline__ void adamw_bias(AdamwStep& h, const AdamwParams& a, float cf) {
-  h.inv1 = 1.f / -expm1f((cf + 1.f) * a.ln_b1);
-  h.inv2 = 1.f / -expm1f((cf + 1.f) * a.ln_b2);
-}
+// Step values of a tensor.
 __device__ __forceinline__ void adamw_rates(AdamwStep& h, const AdamwDesc& d, float cf) {
   const float lr = d.lr_init * expf(cf * d.ln_decay);
   h.rate = lr * h.inv1;
@@ -563,16 +620,17 @@ template <int N>
 __global__ void __launch_bounds__(32 * kAdamwWarps, GS_ADAMW_CTAS)
 k_adamw32(const __grid_constant__ AdamwTable<N> tab, const __grid_constant__ AdamwParams a) {
   GS_PDL_ENTRY_PLAIN();
-  const int c = *(volatile int*)a.state;
-  const float s = a.scale ? *(volatile const float*)a.scale : 1.f;
-  const bool go = fabsf(s) <= 3.402823466e38f;
-  if (go) {
+  __shared__ AdamwHead head;
+  const unsigned ticket = adamw_head(a, head);
+  if (head.go) {
+    const float s = head.s, cf = (float)head.c;
     AdamwStep h;
-    adamw_bias(h, a, (float)c);
+    h.inv1 = head.inv1;
+    h.inv2 = head.inv2;
     int last = -1;
     for (TileWalk<N> w(tab); w.valid(); w.next()) {
       const AdamwDesc& d = tab.t[w.k];
-      if (w.k != last) adamw_rates(h, d, (float)c);
+      if (w.k != last) adamw_rates(h, d, cf);
       last = w.k;
       const long long base = w.base() + (threadIdx.x >> 5) * kAdamwChunk, left = d.count - base;
       if (left >= kAdamwChunk) {
@@ -585,12 +643,39 @@ k_adamw32(const __grid_constant__ AdamwTable<N> tab, const __grid_constant__ Ada
           default: adamw32_chunk<GS_TYPE_F16, true>(d, base, a, h, s); break;
         }
       } else {
-        for (int e = 0; e < left; e += kAdamwBlock)
-          adamw_rest<32>(d, base + e, (int)(left - e < kAdamwBlock ? left - e : kAdamwBlock), a, h, s, 0u);
+        adamw_blocks<32>(d, base, kAdamwChunk, a, h, s, 0u);
       }
     }
   }
-  if (a.advance) adamw_advance(a, c, go);
+  adamw_finish(a, head, ticket);
+}
+
+// Few elements: the time is latency, so every warp has one block, loads its
+// data before it knows the step's values, and runs little code.
+constexpr int kSmallWarps = 4;
+template <int BITS, int N>
+__global__ void __launch_bounds__(32 * kSmallWarps)
+k_adamw_small(const __grid_constant__ AdamwTable<N> tab, const __grid_constant__ AdamwParams a) {
+  GS_PDL_ENTRY_PLAIN();
+  __shared__ AdamwHead head;
+  const TileWalk<N> w(tab);  // here a tile is kSmallWarps blocks
+  const AdamwDesc& d = tab.t[w.k];
+  AdamwBlock<BITS> b;
+  b.rem = 0;
+  if (w.valid()) {
+    const long long base = ((long long)(w.tile - tab.first[w.k]) * kSmallWarps + (threadIdx.x >> 5)) * kAdamwBlock;
+    if (base < d.count) b.load(d, base, (int)(d.count - base < kAdamwBlock ? d.count - base : kAdamwBlock));
+  }
+  const unsigned ticket = adamw_head(a, head);
+  if (head.go && b.rem > 0) {
+    AdamwStep h;
+    h.inv1 = head.inv1;
+    h.inv2 = head.inv2;
+    adamw_rates(h, d, (float)head.c);
+    const unsigned key = mix32(a.seed + kGolden * (unsigned)head.c);
+    b.step(d, a, h, head.s, mix32(key + kGolden * (unsigned)(tab.index0 + w.k)));
+  }
+  adamw_finish(a, head, ticket);
 }
 
 // 8-bit moments. The step's instructions take the SMs about as long as its
@@ -804,25 +889,25 @@ __global__ void __launch_bounds__(32 * kWarps8, GS_ADAMW8_CTAS)
 k_adamw8(const __grid_constant__ AdamwTable<N> tab, const __grid_constant__ AdamwParams a) {
   GS_PDL_ENTRY_PLAIN();
   __shared__ Adamw8Stage stages[kWarps8][2];
-  const int c = *(volatile int*)a.state;
-  const float s = a.scale ? *(volatile const float*)a.scale : 1.f;
-  const bool go = fabsf(s) <= 3.402823466e38f;
-  if (go) {
-    const int lane = threadIdx.x & 31;
+  __shared__ AdamwHead head;
+  const int lane = threadIdx.x & 31;
+  TileWalk<N> w(tab);
+  Adamw8Chunk now = {}, next = {};
+  Adamw8Stage* st = stages[threadIdx.x >> 5];
+  bool more = w.valid();
+  if (more) {
+    now.k = w.k;
+    now.tile = w.base();
+    adamw8_issue(tab.t[now.k], now, st[0], lane);
+  }
+  const unsigned ticket = adamw_head(a, head);
+  if (head.go) {
+    const float s = head.s;
     AdamwStep h;
-    adamw_bias(h, a, (float)c);
-    const unsigned key = mix32(a.seed + kGolden * (unsigned)c);
+    h.inv1 = head.inv1;
+    h.inv2 = head.inv2;
     unsigned tkey = 0u;
-    TileWalk<N> w(tab);
-    Adamw8Chunk now = {}, next = {};
-    Adamw8Stage* st = stages[threadIdx.x >> 5];
     int at = 0, last = -1;
-    bool more = w.valid();
-    if (more) {
-      now.k = w.k;
-      now.tile = w.base();
-      adamw8_issue(tab.t[now.k], now, st[0], lane);
-    }
     while (more) {
       w.next();
       more = w.valid();
@@ -837,8 +922,8 @@ k_adamw8(const __grid_constant__ AdamwTable<N> tab, const __grid_constant__ Adam
       __syncwarp();
       const AdamwDesc& d = tab.t[now.k];
       if (now.k != last) {
-        adamw_rates(h, d, (float)c);
-        tkey = mix32(key + kGolden * (unsigned)(tab.index0 + now.k));
+        adamw_rates(h, d, (float)head.c);
+        tkey = mix32(mix32(a.seed + kGolden * (unsigned)head.c) + kGolden * (unsigned)(tab.index0 + now.k));
         last = now.k;
       }
       if (now.kind != kDirect) {
@@ -852,21 +937,25 @@ k_adamw8(const __grid_constant__ AdamwTable<N> tab, const __grid_constant__ Adam
           default: adamw8_chunk<GS_TYPE_F16, true>(d, now, st[at], a, h, s, tkey, lane); break;
         }
       } else {
-        const long long base = now.tile + (threadIdx.x >> 5) * kChunk8, left = d.count - base;
-        for (int e = 0; e < kChunk8 && e < left; e += kAdamwBlock)
-          adamw_rest<8>(d, base + e, (int)(left - e < kAdamwBlock ? left - e : kAdamwBlock), a, h, s, tkey);
+        adamw_blocks<8>(d, now.tile + (threadIdx.x >> 5) * kChunk8, kChunk8, a, h, s, tkey);
       }
       __syncwarp();  // the stage has been read before it is copied into again
       now = next;
       at ^= 1;
     }
   }
-  if (a.advance) adamw_advance(a, c, go);
+  asm volatile("cp.async.wait_all;" ::: "memory");  // of a step that is skipped
+  adamw_finish(a, head, ticket);
 }
 
 template <int BITS, int N>
 static void launch_adamw_class(const GsAdamwTensor* t, int n, int index0, const AdamwParams& a, cudaStream_t st) {
   static thread_local AdamwTable<N> tab;
+  // one block a warp while that fills the SMs at most GS_ADAMW_SMALL times
+  long long blocks = 0;
+  for (int i = 0; i < n; ++i) blocks += (t[i].count + kAdamwBlock - 1) / kAdamwBlock;
+  const bool small = blocks <= (long long)device_sms() * GS_ADAMW_SMALL;
+  const int tile = small ? kSmallWarps * kAdamwBlock : kAdamwTile;
   int tiles = 0;
   for (int i = 0; i < n; ++i) {
     AdamwDesc& d = tab.t[i];
@@ -891,15 +980,19 @@ static void launch_adamw_class(const GsAdamwTensor* t, int n, int index0, const 
     bits |= (uintptr_t)t[i].mu | (uintptr_t)t[i].nu;
     d.vec = (bits & 15) == 0;
     tab.first[i] = tiles;
-    tiles += (int)((t[i].count + kAdamwTile - 1) / kAdamwTile);
+    tiles += (int)((t[i].count + tile - 1) / tile);
   }
   tab.first[n] = tiles;
   tab.n = n;
   tab.index0 = index0;
-  const int grid = std::max(1, std::min(tiles, device_sms() * (BITS == 8 ? GS_ADAMW8_CTAS : 8)));
   GS_TIMED(BITS == 8 ? "adamw8" : "adamw", st);
-  if (BITS == 8) launch_kernel_plain(k_adamw8<N>, grid, 32 * kWarps8, 0, st, tab, a);
-  else launch_kernel_plain(k_adamw32<N>, grid, 32 * kAdamwWarps, 0, st, tab, a);
+  if (small) {
+    launch_kernel_plain(k_adamw_small<BITS, N>, std::max(1, tiles), 32 * kSmallWarps, 0, st, tab, a);
+  } else if (BITS == 8) {
+    launch_kernel_plain(k_adamw8<N>, std::min(tiles, device_sms() * GS_ADAMW8_CTAS), 32 * kWarps8, 0, st, tab, a);
+  } else {
+    launch_kernel_plain(k_adamw32<N>, std::min(tiles, device_sms() * 8), 32 * kAdamwWarps, 0, st, tab, a);
+  }
 }
 
 constexpr int kAdamwSmall = 8, kAdamwMost = 256;
