@@ -535,15 +535,16 @@ struct AdamwBlock {
   }
 };
 
-// The blocks of [base, base + chunk) that are in the tensor, one by one.
+// A tile's elements behind its `full` whole chunks (those of the first warps),
+// block by block, by the other warps.
 template <int BITS>
-__device__ __forceinline__ void adamw_blocks(const AdamwDesc& d, long long base, int chunk, const AdamwParams& a,
-                                             const AdamwStep& h, float s, unsigned key) {
-  const long long left = d.count - base;
+__device__ __forceinline__ void adamw_blocks(const AdamwDesc& d, long long tile, int full, int warps, int chunk,
+                                             const AdamwParams& a, const AdamwStep& h, float s, unsigned key) {
+  const int end = (int)min(d.count - tile, (long long)kAdamwTile), warp = threadIdx.x >> 5;
 #pragma unroll 1
-  for (int e = 0; e < chunk && e < left; e += kAdamwBlock) {
+  for (int e = full * chunk + (warp - full) * kAdamwBlock; e < end; e += (warps - full) * kAdamwBlock) {
     AdamwBlock<BITS> b;
-    b.load(d, base + e, (int)(left - e < kAdamwBlock ? left - e : kAdamwBlock));
+    b.load(d, tile + e, min(end - e, kAdamwBlock));
     b.step(d, a, h, s, key);
   }
 }
@@ -632,8 +633,9 @@ k_adamw32(const __grid_constant__ AdamwTable<N> tab, const __grid_constant__ Ada
       const AdamwDesc& d = tab.t[w.k];
       if (w.k != last) adamw_rates(h, d, cf);
       last = w.k;
-      const long long base = w.base() + (threadIdx.x >> 5) * kAdamwChunk, left = d.count - base;
-      if (left >= kAdamwChunk) {
+      const int full = (int)min((d.count - w.base()) / kAdamwChunk, (long long)kAdamwWarps);
+      if ((int)(threadIdx.x >> 5) < full) {
+        const long long base = w.base() + (threadIdx.x >> 5) * kAdamwChunk;
         switch (d.grad_type * 2 + d.vec) {
           case 0: adamw32_chunk<GS_TYPE_F32, false>(d, base, a, h, s); break;
           case 1: adamw32_chunk<GS_TYPE_F32, true>(d, base, a, h, s); break;
@@ -643,7 +645,7 @@ k_adamw32(const __grid_constant__ AdamwTable<N> tab, const __grid_constant__ Ada
           default: adamw32_chunk<GS_TYPE_F16, true>(d, base, a, h, s); break;
         }
       } else {
-        adamw_blocks<32>(d, base, kAdamwChunk, a, h, s, 0u);
+        adamw_blocks<32>(d, w.base(), full, kAdamwWarps, kAdamwChunk, a, h, s, 0u);
       }
     }
   }
@@ -787,8 +789,8 @@ __device__ __forceinline__ unsigned half_max2(unsigned x) {
   return x;
 }
 
-// Blocks 2 j and 2 j + 1 of a chunk. ALL: every row active, no copy.
-template <int GT, bool ALL>
+// Blocks 2 j and 2 j + 1 of a chunk. ALL: every row active; COPY: a copy is written.
+template <int GT, bool ALL, bool COPY>
 __device__ __forceinline__ void adamw8_blocks(const AdamwDesc& d, const Adamw8Chunk& c, const Adamw8Stage& st, int j,
                                               unsigned& exps, const AdamwParams& a, const AdamwStep& h, float s,
                                               unsigned key, int lane) {
@@ -827,16 +829,16 @@ __device__ __forceinline__ void adamw8_blocks(const AdamwDesc& d, const Adamw8Ch
       m[4 * i + q] = add_rn(m[4 * i + q], mul_rn(gq, a.omb1));
       v[4 * i + q] = add_rn(v[4 * i + q], mul_rn(mul_rn(gq, gq), a.omb2));
     }
-    if (ALL || c.kind != kNone || d.copy) {
+    if (ALL || COPY || c.kind != kNone) {
       load4<true>(st.p, e, p);
       adamw_param4(p, m + 4 * i, v + 4 * i, h, a, fresh);
-      if (!ALL && c.kind != kAll) {
+      if (!ALL) {
 #pragma unroll
         for (int q = 0; q < 4; ++q)
           if (c.kind == kNone || !((c.act >> (8 * j + 4 * i + q)) & 1u)) fresh[q] = p[q];
       }
       if (ALL || c.kind != kNone) store4<true>(d.param + c.tile, chunk + e, fresh);
-      if (!ALL && d.copy)
+      if (COPY)
         store_copy4<true>(static_cast<char*>(d.copy) + c.tile * 2, chunk + e, d.copy_type, fresh);
     }
   }
@@ -862,11 +864,11 @@ __device__ __forceinline__ void adamw8_blocks(const AdamwDesc& d, const Adamw8Ch
   if ((lane & 3) >> 1 == j) exps = lane < 4 ? both & 0xFFFFu : both >> 16;
 }
 
-template <int GT, bool ALL>
+template <int GT, bool ALL, bool COPY>
 __device__ __forceinline__ void adamw8_chunk(const AdamwDesc& d, const Adamw8Chunk& c, const Adamw8Stage& st,
                                              const AdamwParams& a, const AdamwStep& h, float s, unsigned key, int lane) {
   unsigned exps = 0u;
-  if (!ALL && c.kind == kNone && !d.copy) {
+  if (!ALL && !COPY && c.kind == kNone) {
     // moments and gradients all zero in rows that are not active: nothing changes
     unsigned any = lane < 8 ? c.exps : 0u;
 #pragma unroll
@@ -879,9 +881,21 @@ __device__ __forceinline__ void adamw8_chunk(const AdamwDesc& d, const Adamw8Chu
     if (__all_sync(0xffffffffu, any == 0u)) return;
   }
 #pragma unroll
-  for (int j = 0; j < 2; ++j) adamw8_blocks<GT, ALL>(d, c, st, j, exps, a, h, s, key, lane);
+  for (int j = 0; j < 2; ++j) adamw8_blocks<GT, ALL, COPY>(d, c, st, j, exps, a, h, s, key, lane);
   if (lane < 8)
     ((lane < 4 ? d.mu_exp : d.nu_exp) + c.tile / kAdamwBlock)[(threadIdx.x >> 5) * 4 + (lane & 3)] = (uint8_t)exps;
+}
+
+template <int GT>
+__device__ __forceinline__ void adamw8_typed(const AdamwDesc& d, const Adamw8Chunk& c, const Adamw8Stage& st,
+                                             const AdamwParams& a, const AdamwStep& h, float s, unsigned key, int lane) {
+  if (c.kind == kAll) {
+    if (d.copy) adamw8_chunk<GT, true, true>(d, c, st, a, h, s, key, lane);
+    else adamw8_chunk<GT, true, false>(d, c, st, a, h, s, key, lane);
+  } else {
+    if (d.copy) adamw8_chunk<GT, false, true>(d, c, st, a, h, s, key, lane);
+    else adamw8_chunk<GT, false, false>(d, c, st, a, h, s, key, lane);
+  }
 }
 
 template <int N>
@@ -927,17 +941,12 @@ k_adamw8(const __grid_constant__ AdamwTable<N> tab, const __grid_constant__ Adam
         last = now.k;
       }
       if (now.kind != kDirect) {
-        const bool all = now.kind == kAll && !d.copy;
-        switch (d.grad_type * 2 + all) {
-          case 0: adamw8_chunk<GS_TYPE_F32, false>(d, now, st[at], a, h, s, tkey, lane); break;
-          case 1: adamw8_chunk<GS_TYPE_F32, true>(d, now, st[at], a, h, s, tkey, lane); break;
-          case 2: adamw8_chunk<GS_TYPE_BF16, false>(d, now, st[at], a, h, s, tkey, lane); break;
-          case 3: adamw8_chunk<GS_TYPE_BF16, true>(d, now, st[at], a, h, s, tkey, lane); break;
-          case 4: adamw8_chunk<GS_TYPE_F16, false>(d, now, st[at], a, h, s, tkey, lane); break;
-          default: adamw8_chunk<GS_TYPE_F16, true>(d, now, st[at], a, h, s, tkey, lane); break;
-        }
+        if (d.grad_type == GS_TYPE_F32) adamw8_typed<GS_TYPE_F32>(d, now, st[at], a, h, s, tkey, lane);
+        else if (d.grad_type == GS_TYPE_BF16) adamw8_typed<GS_TYPE_BF16>(d, now, st[at], a, h, s, tkey, lane);
+        else adamw8_typed<GS_TYPE_F16>(d, now, st[at], a, h, s, tkey, lane);
       } else {
-        adamw_blocks<8>(d, now.tile + (threadIdx.x >> 5) * kChunk8, kChunk8, a, h, s, tkey);
+        const int full = d.vec ? (int)min((d.count - now.tile) / kChunk8, (long long)kWarps8) : 0;
+        adamw_blocks<8>(d, now.tile, full, kWarps8, kChunk8, a, h, s, tkey);
       }
       __syncwarp();  // the stage has been read before it is copied into again
       now = next;
