@@ -530,7 +530,8 @@ GS_API int gs_adam_step_flat_device(float* params, const float* grads, float* mu
 /*
  * No reference counterpart (the reference's optimizers are optax.adam over
  * fixed groups): AdamW with decoupled weight decay as optax.adamw defines it,
- * over any number of tensors of any sizes in one launch per 256 of them.
+ * over any number of tensors of any sizes in one launch per 256 of them (128
+ * where the alignment of each differs).
  * With c = state[0] before the call, t = c + 1 and s = *grad_scale (1 if
  * NULL), for every element of every tensor:
  *   g  = s grad;  m' = b1 m + (1 - b1) g;  v' = b2 v + (1 - b2) g^2

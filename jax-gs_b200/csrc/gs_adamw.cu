@@ -53,10 +53,10 @@ static_assert(kAdamwBlock == 128, "a warp holds a block, four elements a lane");
 #define GS_DECODE_UNROLL 2
 #endif
 #ifndef GS_NORM_VECS
-#define GS_NORM_VECS 4
+#define GS_NORM_VECS 2
 #endif
 #ifndef GS_NORM_CTAS
-#define GS_NORM_CTAS 4
+#define GS_NORM_CTAS 8
 #endif
 #ifndef GS_ADAMW_CTAS
 #define GS_ADAMW_CTAS 3
@@ -79,8 +79,13 @@ struct AdamwDesc {
   float lr_init, ln_decay, weight_decay;  // lr = lr_init exp(c ln_decay)
   unsigned width;                         // elements per active flag
   unsigned long long magic;               // ceil(2^64 / width)
-  uint8_t grad_type, copy_type, vec, pad[5];
+  uint8_t grad_type, copy_type, vec;
+  uint8_t skip;  // elements of the first row that lie before the first element (below 4)
+  int index;     // place in the caller's list (the noise key)
 };
+// AdamwDesc::vec: accesses of four elements, of one, and (8-bit moments) of
+// four but for a parameter and fp32 gradient that are not 16-byte aligned.
+constexpr int kScalar = 0, kVec = 1, kLoose = 2;
 
 // Tables travel as kernel parameters (no device copy, nothing to keep alive,
 // and a captured graph holds its own); N is a size class.
@@ -89,8 +94,24 @@ struct AdamwTable {
   AdamwDesc t[N];
   int first[N + 1];  // first tile of each tensor; first[n] = tiles
   int n;
-  int index0;  // place of t[0] in the caller's list (the noise key)
 };
+
+// The tensor of a tile, the last whose first tile is not behind it, by a whole
+// warp: 32 entries at a time (one after the other, 200 tensors' entries took
+// longer to read than their tiles). first[n] is behind every tile.
+template <int N>
+__device__ __forceinline__ int tensor_after(const int (&first)[N], int n, int tile, int k) {
+  const int lane = threadIdx.x & 31;
+  for (int hits = 32; hits == 32; k += hits)
+    hits = __popc(__ballot_sync(0xffffffffu, first[min(k + 1 + lane, n)] <= tile));
+  return k;
+}
+template <int N>
+__device__ __forceinline__ int tensor_of(const int (&first)[N], int n, int tile) {
+  const int lane = threadIdx.x & 31, stride = (n + 31) / 32;
+  const int hits = __popc(__ballot_sync(0xffffffffu, first[min(lane * stride, n)] <= tile));
+  return tensor_after(first, n, tile, max(hits - 1, 0) * stride);
+}
 
 struct AdamwParams {
   float b1, omb1, b2, omb2, eps, ln_b1, ln_b2;
@@ -285,6 +306,7 @@ struct RowPlace {
     return d.width == 1 ? x : __umulhi(x, (unsigned)(d.magic >> 32) + 1u);
   }
   __device__ __forceinline__ void start(const AdamwDesc& d, unsigned long long e) {
+    e += d.skip;
     const unsigned long long row = d.width == 1 ? e : __umul64hi(e, d.magic);
     flags = d.active + row;
     rest = (unsigned)(e - row * d.width);
@@ -593,18 +615,12 @@ struct TileWalk {
   int tile, k;
 
   __device__ __forceinline__ TileWalk(const AdamwTable<N>& t) : tab(t), tile(blockIdx.x), k(0) {
-    // the last tensor whose first tile is not behind this one
-    for (int hi = tab.n; hi - k > 1;) {
-      const int mid = (k + hi) >> 1;
-      if (tab.first[mid] <= tile) k = mid;
-      else hi = mid;
-    }
+    if (valid()) k = tensor_of(tab.first, tab.n, tile);
   }
   __device__ __forceinline__ bool valid() const { return tile < tab.first[tab.n]; }
   __device__ __forceinline__ void next() {
     tile += gridDim.x;
-    if (valid())
-      while (tab.first[k + 1] <= tile) ++k;
+    if (valid() && tab.first[k + 1] <= tile) k = tensor_after(tab.first, tab.n, tile, k);
   }
   // first element of the tile in its tensor
   __device__ __forceinline__ long long base() const { return (long long)(tile - tab.first[k]) * kAdamwTile; }
@@ -636,7 +652,7 @@ k_adamw32(const __grid_constant__ AdamwTable<N> tab, const __grid_constant__ Ada
       const int full = (int)min((d.count - w.base()) / kAdamwChunk, (long long)kAdamwWarps);
       if ((int)(threadIdx.x >> 5) < full) {
         const long long base = w.base() + (threadIdx.x >> 5) * kAdamwChunk;
-        switch (d.grad_type * 2 + d.vec) {
+        switch (d.grad_type * 2 + (d.vec == kVec)) {
           case 0: adamw32_chunk<GS_TYPE_F32, false>(d, base, a, h, s); break;
           case 1: adamw32_chunk<GS_TYPE_F32, true>(d, base, a, h, s); break;
           case 2: adamw32_chunk<GS_TYPE_BF16, false>(d, base, a, h, s); break;
@@ -675,7 +691,7 @@ k_adamw_small(const __grid_constant__ AdamwTable<N> tab, const __grid_constant__
     h.inv2 = head.inv2;
     adamw_rates(h, d, (float)head.c);
     const unsigned key = mix32(a.seed + kGolden * (unsigned)head.c);
-    b.step(d, a, h, head.s, mix32(key + kGolden * (unsigned)(tab.index0 + w.k)));
+    b.step(d, a, h, head.s, mix32(key + kGolden * (unsigned)d.index));
   }
   adamw_finish(a, head, ticket);
 }
@@ -698,6 +714,10 @@ struct __align__(16) Adamw8Stage {
   uint8_t mu[kChunk8], nu[kChunk8];
 };
 
+__device__ __forceinline__ void cp_async4(void* dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"((unsigned)__cvta_generic_to_shared(dst)), "l"(src)
+               : "memory");
+}
 __device__ __forceinline__ void cp_async16(void* dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((unsigned)__cvta_generic_to_shared(dst)), "l"(src)
                : "memory");
@@ -734,15 +754,21 @@ __device__ __forceinline__ int chunk_rows(const AdamwDesc& d, const RowPlace& at
 __device__ __forceinline__ void adamw8_issue(const AdamwDesc& d, Adamw8Chunk& c, Adamw8Stage& st, int lane) {
   const int chunk = (threadIdx.x >> 5) * kChunk8;
   c.kind = kDirect;
-  if (d.vec && d.count - c.tile >= chunk + kChunk8) {
+  if (d.vec != kScalar && d.count - c.tile >= chunk + kChunk8) {
     const int two = d.grad_type == GS_TYPE_F32 ? 2 : 1;
-    const char* g = static_cast<const char*>(d.grad) + (c.tile << two) + (unsigned)((chunk << two) + 16 * lane);
-    char* sg = reinterpret_cast<char*>(st.g) + 16 * lane;
-    cp_async16(sg, g);
-    cp_async16(sg + 512, g + 512);
-    if (two == 2) {
-      cp_async16(sg + 1024, g + 1024);
-      cp_async16(sg + 1536, g + 1536);
+    if (d.vec == kVec) {
+      const char* g = static_cast<const char*>(d.grad) + (c.tile << two) + (unsigned)((chunk << two) + 16 * lane);
+      char* sg = reinterpret_cast<char*>(st.g) + 16 * lane;
+      cp_async16(sg, g);
+      cp_async16(sg + 512, g + 512);
+      if (two == 2) {
+        cp_async16(sg + 1024, g + 1024);
+        cp_async16(sg + 1536, g + 1536);
+      }
+    } else {
+      const float* g = static_cast<const float*>(d.grad) + c.tile + (unsigned)(chunk + lane);
+#pragma unroll
+      for (int n = 0; n < kChunk8 / 32; ++n) cp_async4(st.g + lane + 32 * n, g + 32 * n);
     }
     cp_async16(st.mu + 16 * lane, static_cast<const uint8_t*>(d.mu) + c.tile + (unsigned)(chunk + 16 * lane));
     cp_async16(st.nu + 16 * lane, static_cast<const uint8_t*>(d.nu) + c.tile + (unsigned)(chunk + 16 * lane));
@@ -760,10 +786,14 @@ __device__ __forceinline__ void adamw8_issue(const AdamwDesc& d, Adamw8Chunk& c,
       }
     }
     if (c.kind != kNone || d.copy) {
-      const char* p = reinterpret_cast<const char*>(d.param + c.tile) + (unsigned)(4 * chunk + 16 * lane);
-      char* sp = reinterpret_cast<char*>(st.p) + 16 * lane;
+      const float* p = d.param + c.tile + (unsigned)chunk;
+      if (d.vec == kVec) {
 #pragma unroll
-      for (int n = 0; n < 4; ++n) cp_async16(sp + 512 * n, p + 512 * n);
+        for (int n = 0; n < 4; ++n) cp_async16(st.p + 4 * lane + 128 * n, p + 4 * lane + 128 * n);
+      } else {
+#pragma unroll
+        for (int n = 0; n < kChunk8 / 32; ++n) cp_async4(st.p + lane + 32 * n, p + lane + 32 * n);
+      }
     }
   }
   asm volatile("cp.async.commit_group;" ::: "memory");
@@ -789,9 +819,10 @@ __device__ __forceinline__ unsigned half_max2(unsigned x) {
   return x;
 }
 
-// Blocks 2 j and 2 j + 1 of a chunk. ALL: every row active; COPY: a copy is written.
-template <int GT, bool ALL, bool COPY>
-__device__ __forceinline__ void adamw8_blocks(const AdamwDesc& d, const Adamw8Chunk& c, const Adamw8Stage& st, int j,
+// Blocks 2 j and 2 j + 1 of a chunk. ALL: every row active; COPY: a copy is
+// written; LOOSE: the parameter is not 16-byte aligned.
+template <int GT, bool ALL, bool COPY, bool LOOSE>
+__device__ __forceinline__ void adamw8_blocks(const AdamwDesc& d, const Adamw8Chunk& c, Adamw8Stage& st, int j,
                                               unsigned& exps, const AdamwParams& a, const AdamwStep& h, float s,
                                               unsigned key, int lane) {
   const int src = 2 * j + (lane >> 4);  // the half's block
@@ -837,7 +868,10 @@ __device__ __forceinline__ void adamw8_blocks(const AdamwDesc& d, const Adamw8Ch
         for (int q = 0; q < 4; ++q)
           if (c.kind == kNone || !((c.act >> (8 * j + 4 * i + q)) & 1u)) fresh[q] = p[q];
       }
-      if (ALL || c.kind != kNone) store4<true>(d.param + c.tile, chunk + e, fresh);
+      if (ALL || c.kind != kNone) {
+        if (LOOSE) store4<true>(st.p, e, fresh);  // stored from there when the chunk is done
+        else store4<true>(d.param + c.tile, chunk + e, fresh);
+      }
       if (COPY)
         store_copy4<true>(static_cast<char*>(d.copy) + c.tile * 2, chunk + e, d.copy_type, fresh);
     }
@@ -864,8 +898,8 @@ __device__ __forceinline__ void adamw8_blocks(const AdamwDesc& d, const Adamw8Ch
   if ((lane & 3) >> 1 == j) exps = lane < 4 ? both & 0xFFFFu : both >> 16;
 }
 
-template <int GT, bool ALL, bool COPY>
-__device__ __forceinline__ void adamw8_chunk(const AdamwDesc& d, const Adamw8Chunk& c, const Adamw8Stage& st,
+template <int GT, bool ALL, bool COPY, bool LOOSE>
+__device__ __forceinline__ void adamw8_chunk(const AdamwDesc& d, const Adamw8Chunk& c, Adamw8Stage& st,
                                              const AdamwParams& a, const AdamwStep& h, float s, unsigned key, int lane) {
   unsigned exps = 0u;
   if (!ALL && !COPY && c.kind == kNone) {
@@ -881,20 +915,26 @@ __device__ __forceinline__ void adamw8_chunk(const AdamwDesc& d, const Adamw8Chu
     if (__all_sync(0xffffffffu, any == 0u)) return;
   }
 #pragma unroll
-  for (int j = 0; j < 2; ++j) adamw8_blocks<GT, ALL, COPY>(d, c, st, j, exps, a, h, s, key, lane);
+  for (int j = 0; j < 2; ++j) adamw8_blocks<GT, ALL, COPY, LOOSE>(d, c, st, j, exps, a, h, s, key, lane);
   if (lane < 8)
     ((lane < 4 ? d.mu_exp : d.nu_exp) + c.tile / kAdamwBlock)[(threadIdx.x >> 5) * 4 + (lane & 3)] = (uint8_t)exps;
+  if (LOOSE && (ALL || c.kind != kNone)) {
+    __syncwarp();
+    float* const param = d.param + c.tile + (threadIdx.x >> 5) * kChunk8 + lane;
+#pragma unroll
+    for (int n = 0; n < kChunk8 / 32; ++n) param[32 * n] = st.p[lane + 32 * n];
+  }
 }
 
-template <int GT>
-__device__ __forceinline__ void adamw8_typed(const AdamwDesc& d, const Adamw8Chunk& c, const Adamw8Stage& st,
+template <int GT, bool LOOSE>
+__device__ __forceinline__ void adamw8_typed(const AdamwDesc& d, const Adamw8Chunk& c, Adamw8Stage& st,
                                              const AdamwParams& a, const AdamwStep& h, float s, unsigned key, int lane) {
   if (c.kind == kAll) {
-    if (d.copy) adamw8_chunk<GT, true, true>(d, c, st, a, h, s, key, lane);
-    else adamw8_chunk<GT, true, false>(d, c, st, a, h, s, key, lane);
+    if (d.copy) adamw8_chunk<GT, true, true, LOOSE>(d, c, st, a, h, s, key, lane);
+    else adamw8_chunk<GT, true, false, LOOSE>(d, c, st, a, h, s, key, lane);
   } else {
-    if (d.copy) adamw8_chunk<GT, false, true>(d, c, st, a, h, s, key, lane);
-    else adamw8_chunk<GT, false, false>(d, c, st, a, h, s, key, lane);
+    if (d.copy) adamw8_chunk<GT, false, true, LOOSE>(d, c, st, a, h, s, key, lane);
+    else adamw8_chunk<GT, false, false, LOOSE>(d, c, st, a, h, s, key, lane);
   }
 }
 
@@ -937,15 +977,16 @@ k_adamw8(const __grid_constant__ AdamwTable<N> tab, const __grid_constant__ Adam
       const AdamwDesc& d = tab.t[now.k];
       if (now.k != last) {
         adamw_rates(h, d, (float)head.c);
-        tkey = mix32(mix32(a.seed + kGolden * (unsigned)head.c) + kGolden * (unsigned)(tab.index0 + now.k));
+        tkey = mix32(mix32(a.seed + kGolden * (unsigned)head.c) + kGolden * (unsigned)d.index);
         last = now.k;
       }
       if (now.kind != kDirect) {
-        if (d.grad_type == GS_TYPE_F32) adamw8_typed<GS_TYPE_F32>(d, now, st[at], a, h, s, tkey, lane);
-        else if (d.grad_type == GS_TYPE_BF16) adamw8_typed<GS_TYPE_BF16>(d, now, st[at], a, h, s, tkey, lane);
-        else adamw8_typed<GS_TYPE_F16>(d, now, st[at], a, h, s, tkey, lane);
+        if (d.vec == kLoose) adamw8_typed<GS_TYPE_F32, true>(d, now, st[at], a, h, s, tkey, lane);
+        else if (d.grad_type == GS_TYPE_F32) adamw8_typed<GS_TYPE_F32, false>(d, now, st[at], a, h, s, tkey, lane);
+        else if (d.grad_type == GS_TYPE_BF16) adamw8_typed<GS_TYPE_BF16, false>(d, now, st[at], a, h, s, tkey, lane);
+        else adamw8_typed<GS_TYPE_F16, false>(d, now, st[at], a, h, s, tkey, lane);
       } else {
-        const int full = d.vec ? (int)min((d.count - now.tile) / kChunk8, (long long)kWarps8) : 0;
+        const int full = d.vec != kScalar ? (int)min((d.count - now.tile) / kChunk8, (long long)kWarps8) : 0;
         adamw_blocks<8>(d, now.tile, full, kWarps8, kChunk8, a, h, s, tkey);
       }
       __syncwarp();  // the stage has been read before it is copied into again
@@ -957,6 +998,65 @@ k_adamw8(const __grid_constant__ AdamwTable<N> tab, const __grid_constant__ Adam
   adamw_finish(a, head, ticket);
 }
 
+// One entry for a tensor, or two: with 32-bit moments a tensor whose arrays
+// all lie the same elements behind a 16-byte boundary (the groups of a flat
+// buffer of odd capacity) is cut after the elements up to the next one, and
+// the rest is accessed four elements at a time.
+static int describe(const GsAdamwTensor& t, int index, int bits, AdamwDesc out[2]) {
+  AdamwDesc d;
+  d.param = t.param;
+  d.grad = t.grad;
+  d.mu = t.mu;
+  d.nu = t.nu;
+  d.mu_exp = t.mu_exp;
+  d.nu_exp = t.nu_exp;
+  d.copy = t.copy;
+  d.active = t.active;
+  d.count = t.count;
+  d.lr_init = t.lr_init;
+  d.ln_decay = (float)(std::log((double)t.decay_rate) / (double)t.transition_steps);
+  d.weight_decay = t.weight_decay;
+  d.width = (unsigned)t.width;
+  d.magic = t.width > 1 ? ~0ull / (unsigned)t.width + 1ull : 0ull;
+  d.grad_type = (uint8_t)t.grad_type;
+  d.copy_type = (uint8_t)t.copy_type;
+  d.skip = 0;
+  d.index = index;
+  const uintptr_t p = (uintptr_t)t.param, g = (uintptr_t)t.grad, m = (uintptr_t)t.mu, v = (uintptr_t)t.nu,
+                  c = (uintptr_t)t.copy;
+  const bool f32 = t.grad_type == GS_TYPE_F32;
+  d.vec = kScalar;
+  if (bits == 8) {
+    if (((m | v) & 15) == 0 && (c & 7) == 0) d.vec = ((p | g) & 15) == 0 ? kVec : (f32 ? kLoose : kScalar);
+    out[0] = d;
+    return 1;
+  }
+  const uintptr_t behind = p / 4 & 3;  // elements behind a boundary
+  const bool same = (m / 4 & 3) == behind && (v / 4 & 3) == behind &&
+                    (f32 ? (g / 4 & 3) == behind : (g & 1) == 0 && (g / 2 & 3) == behind) &&
+                    (!t.copy || (c / 2 & 3) == behind);
+  out[0] = d;
+  if (!same) return 1;
+  if (behind == 0) {
+    out[0].vec = kVec;
+    return 1;
+  }
+  const int64_t head = 4 - (int64_t)behind;
+  if (t.count <= head) return 1;
+  out[0].count = head;
+  d.param += head;
+  d.grad = static_cast<const char*>(d.grad) + head * (f32 ? 4 : 2);
+  d.mu = static_cast<float*>(d.mu) + head;
+  d.nu = static_cast<float*>(d.nu) + head;
+  if (d.copy) d.copy = static_cast<char*>(d.copy) + head * 2;
+  d.count -= head;
+  d.skip = (uint8_t)head;
+  d.vec = kVec;
+  out[1] = d;
+  return 2;
+}
+
+// Tensors t[0 .. n), the caller's index0-th and on, in at most N entries.
 template <int BITS, int N>
 static void launch_adamw_class(const GsAdamwTensor* t, int n, int index0, const AdamwParams& a, cudaStream_t st) {
   static thread_local AdamwTable<N> tab;
@@ -965,35 +1065,19 @@ static void launch_adamw_class(const GsAdamwTensor* t, int n, int index0, const 
   for (int i = 0; i < n; ++i) blocks += (t[i].count + kAdamwBlock - 1) / kAdamwBlock;
   const bool small = blocks <= (long long)device_sms() * GS_ADAMW_SMALL;
   const int tile = small ? kSmallWarps * kAdamwBlock : kAdamwTile;
-  int tiles = 0;
+  int tiles = 0, entries = 0;
   for (int i = 0; i < n; ++i) {
-    AdamwDesc& d = tab.t[i];
-    d.param = t[i].param;
-    d.grad = t[i].grad;
-    d.mu = t[i].mu;
-    d.nu = t[i].nu;
-    d.mu_exp = t[i].mu_exp;
-    d.nu_exp = t[i].nu_exp;
-    d.copy = t[i].copy;
-    d.active = t[i].active;
-    d.count = t[i].count;
-    d.lr_init = t[i].lr_init;
-    d.ln_decay = (float)(std::log((double)t[i].decay_rate) / (double)t[i].transition_steps);
-    d.weight_decay = t[i].weight_decay;
-    d.width = (unsigned)t[i].width;
-    d.grad_type = (uint8_t)t[i].grad_type;
-    d.copy_type = (uint8_t)t[i].copy_type;
-    d.magic = t[i].width > 1 ? ~0ull / (unsigned)t[i].width + 1ull : 0ull;
-    const size_t g4 = t[i].grad_type == GS_TYPE_F32 ? 16 : 8;
-    uintptr_t bits = (uintptr_t)t[i].param | ((uintptr_t)t[i].copy * 2) | ((uintptr_t)t[i].grad * (BITS == 8 ? 1 : 16 / g4));
-    bits |= (uintptr_t)t[i].mu | (uintptr_t)t[i].nu;
-    d.vec = (bits & 15) == 0;
-    tab.first[i] = tiles;
-    tiles += (int)((t[i].count + tile - 1) / tile);
+    AdamwDesc d[2];
+    const int k = describe(t[i], index0 + i, BITS, d);
+    if (small && k == 2) d[0].count = t[i].count;  // element by element all the same
+    for (int j = 0; j < (small ? 1 : k); ++j) {
+      tab.t[entries] = d[j];
+      tab.first[entries++] = tiles;
+      tiles += (int)((d[j].count + tile - 1) / tile);
+    }
   }
-  tab.first[n] = tiles;
-  tab.n = n;
-  tab.index0 = index0;
+  tab.first[entries] = tiles;
+  tab.n = entries;
   GS_TIMED(BITS == 8 ? "adamw8" : "adamw", st);
   if (small) {
     launch_kernel_plain(k_adamw_small<BITS, N>, std::max(1, tiles), 32 * kSmallWarps, 0, st, tab, a);
@@ -1004,7 +1088,25 @@ static void launch_adamw_class(const GsAdamwTensor* t, int n, int index0, const 
   }
 }
 
-constexpr int kAdamwSmall = 8, kAdamwMost = 256;
+constexpr int kAdamwSmall = 12, kAdamwMost = 256;  // entries of a table
+
+template <int BITS>
+static void launch_adamw_bits(const GsAdamwTensor* tensors, int n, AdamwParams& a, cudaStream_t st) {
+  int at = 0;
+  do {
+    // as many tensors as have entries
+    int entries = 0, take = 0;
+    for (AdamwDesc d[2]; at + take < n; ++take) {
+      const int k = describe(tensors[at + take], 0, BITS, d);
+      if (entries + k > kAdamwMost) break;
+      entries += k;
+    }
+    a.advance = at + take >= n;
+    if (entries <= kAdamwSmall) launch_adamw_class<BITS, kAdamwSmall>(tensors + at, take, at, a, st);
+    else launch_adamw_class<BITS, kAdamwMost>(tensors + at, take, at, a, st);
+    at += take;
+  } while (at < n);
+}
 
 void launch_adamw(const GsAdamwTensor* tensors, int n, const GsAdamwConfig& cfg, const float* scale, int* state,
                   cudaStream_t st) {
@@ -1020,19 +1122,8 @@ void launch_adamw(const GsAdamwTensor* tensors, int n, const GsAdamwConfig& cfg,
   a.fine_root = a.eps < 0x1p-39f;
   a.scale = scale;
   a.state = state;
-  int at = 0;
-  do {
-    const int take = std::min(n - at, kAdamwMost);
-    a.advance = at + take >= n;
-    if (cfg.moment_bits == 8) {
-      if (take <= kAdamwSmall) launch_adamw_class<8, kAdamwSmall>(tensors + at, take, at, a, st);
-      else launch_adamw_class<8, kAdamwMost>(tensors + at, take, at, a, st);
-    } else {
-      if (take <= kAdamwSmall) launch_adamw_class<32, kAdamwSmall>(tensors + at, take, at, a, st);
-      else launch_adamw_class<32, kAdamwMost>(tensors + at, take, at, a, st);
-    }
-    at += take;
-  } while (at < n);
+  if (cfg.moment_bits == 8) launch_adamw_bits<8>(tensors, n, a, st);
+  else launch_adamw_bits<32>(tensors, n, a, st);
 }
 
 // ---------------------------------------------------------------------------
@@ -1054,9 +1145,10 @@ struct GradTable {
   int n;
 };
 
-// A tile is 16 KB of a tensor counted from the 16-byte boundary at or before
-// its first element, 64 bytes a thread in 16-byte loads; only the vectors
+// A tile is 8 KB of a tensor counted from the 16-byte boundary at or before
+// its first element, 32 bytes a thread in 16-byte loads; only the vectors
 // that hold both the tensor's elements and others are read one by one.
+constexpr int kNormSmall = 8, kNormMost = 1024, kNormGrid = 1184;  // 8 CTAs an SM
 constexpr int kNormVecs = GS_NORM_VECS;
 constexpr int kNormTileBytes = 256 * 16 * kNormVecs;
 
@@ -1127,14 +1219,16 @@ k_grad_norm(const __grid_constant__ GradTable<N> tab, double* __restrict__ parti
   __shared__ bool s_last;
   double sums[4] = {0.0, 0.0, 0.0, 0.0};
   const int tiles = tab.first[tab.n];
-  int k = 0;
-  for (int hi = tab.n; hi - k > 1;) {
-    const int mid = (k + hi) >> 1;
-    if (tab.first[mid] <= (int)blockIdx.x) k = mid;
-    else hi = mid;
-  }
-  for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
-    while (tab.first[k + 1] <= tile) ++k;
+  // Many tensors: consecutive tiles, so that a CTA reads few entries of the
+  // table (each new one is a miss of the constant cache: 197 tensors of 100 MB
+  // took 39 us in strides and 26 us so). Few: strides, which end more evenly.
+  constexpr bool kRange = N > kNormSmall;
+  const int t0 = kRange ? (int)((long long)tiles * blockIdx.x / gridDim.x) : (int)blockIdx.x;
+  const int t1 = kRange ? (int)((long long)tiles * (blockIdx.x + 1) / gridDim.x) : tiles;
+  const int step = kRange ? 1 : (int)gridDim.x;
+  int k = t0 < t1 ? tensor_of(tab.first, tab.n, t0) : 0;
+  for (int tile = t0; tile < t1; tile += step) {
+    if (tab.first[k + 1] <= tile) k = tensor_after(tab.first, tab.n, tile, k);
     const GradDesc& d = tab.t[k];
     const long long t = tile - tab.first[k];
     if (d.type == GS_TYPE_F32) norm_tile<GS_TYPE_F32>(d, t, sums);
@@ -1183,7 +1277,6 @@ static int fill_grad_table(const GsGradTensor* t, int n, GradTable<N>& tab) {
   return tiles;
 }
 
-constexpr int kNormSmall = 8, kNormMost = 1024, kNormGrid = 1184;
 
 size_t grad_norm_workspace_bytes(int n) {
   const size_t launches = n > 0 ? ((size_t)n + kNormMost - 1) / kNormMost : 1;
@@ -1228,12 +1321,18 @@ void launch_grad_norm(const GsGradTensor* tensors, int n, float max_norm, const 
 __device__ __forceinline__ void store_value(float* p, float x) { *p = x; }
 __device__ __forceinline__ void store_value(__nv_bfloat16* p, float x) { *p = __float2bfloat16_rn(x); }
 
-__device__ __forceinline__ void store_values4(float* p, const float x[4]) {
-  *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]);
+__device__ __forceinline__ void store_values8(float* p, const float x[8]) {
+  reinterpret_cast<float4*>(p)[0] = make_float4(x[0], x[1], x[2], x[3]);
+  reinterpret_cast<float4*>(p)[1] = make_float4(x[4], x[5], x[6], x[7]);
 }
-__device__ __forceinline__ void store_values4(__nv_bfloat16* p, const float x[4]) {
-  const __nv_bfloat162 a = __floats2bfloat162_rn(x[0], x[1]), b = __floats2bfloat162_rn(x[2], x[3]);
-  *reinterpret_cast<uint2*>(p) = make_uint2(*reinterpret_cast<const unsigned*>(&a), *reinterpret_cast<const unsigned*>(&b));
+__device__ __forceinline__ void store_values8(__nv_bfloat16* p, const float x[8]) {
+  unsigned w[4];
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    const __nv_bfloat162 a = __floats2bfloat162_rn(x[2 * q], x[2 * q + 1]);
+    w[q] = *reinterpret_cast<const unsigned*>(&a);
+  }
+  *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
 }
 
 template <bool SIGNED>
@@ -1246,7 +1345,7 @@ __device__ __forceinline__ void values4(unsigned w, int field, float x[4]) {
   }
 }
 
-// VEC: four codes of each moment a thread and turn, 2 turns in flight; else one.
+// VEC: eight codes of each moment a thread, U times in flight; else one.
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(256)
 k_moments8_decode(const uint8_t* __restrict__ mu, const uint8_t* __restrict__ nu, const uint8_t* __restrict__ mu_exp,
@@ -1257,33 +1356,35 @@ k_moments8_decode(const uint8_t* __restrict__ mu, const uint8_t* __restrict__ nu
   long long i = blockIdx.x * 256ll + threadIdx.x;
   if (VEC) {
     constexpr int U = GS_DECODE_UNROLL;
-    const long long n4 = count / 4;
-    for (; i < n4; i += U * stride) {
-      unsigned wm[U], wv[U];
+    const long long n8 = count / 8;
+    for (; i < n8; i += U * stride) {
+      uint2 wm[U], wv[U];
       int fm[U], fv[U];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         const long long k = i + u * stride;
-        if (k < n4) {
-          wm[u] = reinterpret_cast<const unsigned*>(mu)[k];
-          wv[u] = reinterpret_cast<const unsigned*>(nu)[k];
-          fm[u] = mu_exp[k / (kAdamwBlock / 4)];
-          fv[u] = nu_exp[k / (kAdamwBlock / 4)];
+        if (k < n8) {
+          wm[u] = reinterpret_cast<const uint2*>(mu)[k];
+          wv[u] = reinterpret_cast<const uint2*>(nu)[k];
+          fm[u] = mu_exp[k / (kAdamwBlock / 8)];
+          fv[u] = nu_exp[k / (kAdamwBlock / 8)];
         }
       }
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         const long long k = i + u * stride;
-        if (k < n4) {
-          float x[4];
-          values4<true>(wm[u], fm[u], x);
-          store_values4(mu_out + 4 * k, x);
-          values4<false>(wv[u], fv[u], x);
-          store_values4(nu_out + 4 * k, x);
+        if (k < n8) {
+          float x[8];
+          values4<true>(wm[u].x, fm[u], x);
+          values4<true>(wm[u].y, fm[u], x + 4);
+          store_values8(mu_out + 8 * k, x);
+          values4<false>(wv[u].x, fv[u], x);
+          values4<false>(wv[u].y, fv[u], x + 4);
+          store_values8(nu_out + 8 * k, x);
         }
       }
     }
-    i = 4 * n4 + blockIdx.x * 256ll + threadIdx.x;  // the last few
+    i = 8 * n8 + blockIdx.x * 256ll + threadIdx.x;  // the last few
   }
   for (; i < count; i += stride) {
     const int fm = mu_exp[i / kAdamwBlock], fv = nu_exp[i / kAdamwBlock];
@@ -1331,9 +1432,8 @@ k_moments8_encode(const float* __restrict__ mu, const float* __restrict__ nu, lo
 
 void launch_moments8_decode(const uint8_t* mu, const uint8_t* nu, const uint8_t* mu_exp, const uint8_t* nu_exp,
                             long long count, int type, void* mu_out, void* nu_out, cudaStream_t st) {
-  const uintptr_t bits = (uintptr_t)mu_out | (uintptr_t)nu_out;
-  const bool vec = (bits & (type == GS_TYPE_F32 ? 15 : 7)) == 0;  // the codes are 4-byte aligned
-  const long long items = vec ? count / 4 + 3 : count;
+  const bool vec = (((uintptr_t)mu_out | (uintptr_t)nu_out) & 15) == 0 && (((uintptr_t)mu | (uintptr_t)nu) & 7) == 0;
+  const long long items = vec ? count / 8 + 7 : count;
   const int grid = (int)std::min((items + 255) / 256, (long long)device_sms() * 8);
   GS_TIMED("moments8_decode", st);
   auto launch = [&](auto kernel, auto* m, auto* v) {
