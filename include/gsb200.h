@@ -628,7 +628,7 @@ GS_API size_t gs_grad_norm_workspace_bytes(int n_tensors);
 /*
  * 8-bit moments to values (type GS_TYPE_F32 or GS_TYPE_BF16, both exact but
  * for values below the type's smallest) and back (to nearest, halves up;
- * values that came from codes are kept exactly). count elements in
+ * the values of a block's codes are kept exactly). count elements in
  * ceil(count / 128) blocks; mu, nu, mu_exp, nu_exp as in GsAdamwTensor.
  */
 GS_API int gs_moments8_decode(const uint8_t* mu, const uint8_t* nu, const uint8_t* mu_exp, const uint8_t* nu_exp,

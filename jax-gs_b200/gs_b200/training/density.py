@@ -56,10 +56,21 @@ def densify_and_prune(state: DensityState, rng_key: Union[int, torch.Generator, 
                               device=dev)
         b["info"] = torch.zeros(4, dtype=torch.int32, device=dev)
     P = _lib.ptr
-    _lib.call("gs_densify_and_prune", P(state.params), P(state.mu), P(state.nu), state.n, state.sh_k,
+    mu, nu = state.mu, state.nu
+    if state.moments8 is not None:
+        # 8-bit moments move between blocks with other exponents: as values,
+        # rounded to nearest where a block has changed
+        flat = state.moments8.values()
+        mu, nu = (torch.cat(state.moments8.split(t)) for t in flat)
+    _lib.call("gs_densify_and_prune", P(state.params), P(mu), P(nu), state.n, state.sh_k,
               P(state.active_mask.view(torch.uint8)), P(state.grad_accum), P(state.denom), P(state.max_radii),
               P(noise), int(bool(densify_enabled)), float(grad_threshold), float(min_opacity), float(extent),
               float(max_screen_size), P(b["ws"]), b["ws"].numel(), P(b["info"]), _lib.stream(dev))
+    if state.moments8 is not None:
+        for t, moved in zip(flat, (mu, nu)):
+            for part, (lo, hi) in zip(state.moments8.split(t), state.segments):
+                part.copy_(moved[lo:hi])
+        state.moments8.set_values(*flat)
     state.densify_info = b["info"]
     return state
 
@@ -78,6 +89,8 @@ def gather_moments(state: DensityState, group) -> None:
     sum over the ranks (exact: one nonzero term per entry) leaves every rank
     with the moments optax would hold on each pmap replica."""
     import torch.distributed as dist
+    if state.moments8 is not None:
+        raise ValueError("8-bit moments are whole on every rank (fused=False)")
     world, rank = dist.get_world_size(group), dist.get_rank(group)
     foreign = dp_owner(state.n, world, state.device) != rank
     widths = [3, 3, 4, 1, 3 * state.sh_k]
@@ -94,7 +107,7 @@ def update_from_rank0(state: DensityState, group, update: Callable[[DensityState
     (train_parallel.py:269-283: unreplicate_tree -> density_step /
     opacity_reset_step -> replicate_tree). With fused=True the moments are
     first gathered (gather_moments). Every rank takes the same collective
-    steps; only rank 0 runs `update`. Copied from rank 0: params, mu, nu,
+    steps; only rank 0 runs `update`. Copied from rank 0: params, the moments,
     active_mask, grad_accum, denom, max_radii and densify_info."""
     import torch.distributed as dist
     if fused:
@@ -105,7 +118,7 @@ def update_from_rank0(state: DensityState, group, update: Callable[[DensityState
     info = getattr(state, "densify_info", None)
     if info is None:
         info = state.densify_info = torch.zeros(4, dtype=torch.int32, device=state.device)
-    for t in (state.params, state.mu, state.nu, state.active_mask.view(torch.uint8), state.grad_accum,
+    for t in (state.params, *state.moment_buffers(), state.active_mask.view(torch.uint8), state.grad_accum,
               state.denom, state.max_radii, info):
         dist.broadcast(t, src=src, group=group)
     return state

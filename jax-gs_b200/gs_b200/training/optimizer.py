@@ -90,24 +90,31 @@ def _check_overlap(written: Sequence[Tuple[str, torch.Tensor]], read: Sequence[T
             end_r, name_r = b, name
 
 
+def _stream(device: torch.device) -> int:
+    """The current stream's handle, without building torch's Stream object (2 us of a 5 us call)."""
+    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+    return raw(device.index) if raw is not None else _lib.stream(device)
+
+
 class _Plan:
     """The device, and the plan's own tensors kept from reuse on the streams that use them."""
 
     def __init__(self, device: torch.device):
         self.device = device
         self._owned: List[torch.Tensor] = []
-        self._streams = {torch.cuda.current_stream(device).cuda_stream}
+        self._streams = {_stream(device)}
 
-    def _stream(self) -> int:
-        s = torch.cuda.current_stream(self.device)
-        if s.cuda_stream not in self._streams and not torch.cuda.is_current_stream_capturing():
-            for t in self._owned:
-                t.record_stream(s)
-            self._streams.add(s.cuda_stream)
-        return s.cuda_stream
+    def _own(self, *tensors: torch.Tensor) -> None:
+        self._owned += tensors
 
     def _call(self, fn: str, *args) -> None:
-        st = self._stream()
+        """One library call on the current stream of the plan's device."""
+        st = _stream(self.device)
+        if st not in self._streams and not torch.cuda.is_current_stream_capturing():
+            s = torch.cuda.current_stream(self.device)
+            for t in self._owned:
+                t.record_stream(s)
+            self._streams.add(st)
         if torch.cuda.current_device() == self.device.index:
             _lib.call(fn, *args, st)
         else:
@@ -143,17 +150,18 @@ class GradNorm(_Plan):
         self._buf = torch.zeros(4, dtype=torch.float32, device=self.device)  # GsGradNorm
         self._ws = torch.empty(_lib.lib().gs_grad_norm_workspace_bytes(len(grads)), dtype=torch.uint8,
                                device=self.device)
-        self._owned = [self._buf, self._ws]
+        self._own(self._buf, self._ws)
         self.out = self._buf[:2]
         self.norm, self.scale = self._buf[0], self._buf[1]
+        self._args = (self._table, len(self._table), self.max_norm, _lib.ptr(self.unscale), self._buf.data_ptr(),
+                      self._ws.data_ptr(), self._ws.numel())
 
     def __call__(self) -> torch.Tensor:
-        self._call("gs_grad_norm", self._table, len(self._table), self.max_norm, _lib.ptr(self.unscale),
-                   self._buf.data_ptr(), self._ws.data_ptr(), self._ws.numel())
+        self._call("gs_grad_norm", *self._args)
         return self.out
 
 
-class Moments8:
+class Moments8(_Plan):
     """Both Adam moments of a list of tensors as 8-bit codes with one exponent
     byte for each 128 elements (the format of gs_adamw_step), in flat buffers
     in which every tensor starts at a multiple of 128 elements. `sizes` are the
@@ -187,30 +195,27 @@ class Moments8:
             if t.data_ptr() % 4:
                 raise ValueError(f"{name}: not 4-byte aligned")
         self.mu, self.nu, self.mu_exp, self.nu_exp = given
-        self.device = self.mu.device
+        super().__init__(self.mu.device)
+        self._own(*given)
+        self._codes = tuple(t.data_ptr() for t in given)
 
     def values(self, dtype: torch.dtype = torch.float32) -> Tuple[torch.Tensor, torch.Tensor]:
         """(mu, nu) that the codes stand for, in the layout of the flat buffers
         (0 between the tensors), in float32 or bfloat16 (exact in both)."""
         if dtype not in (torch.float32, torch.bfloat16):
             raise ValueError("dtype must be float32 or bfloat16")
-        out = torch.empty((2, self.total), dtype=dtype, device=self.device)
-        with torch.cuda.device(self.device):
-            _lib.call("gs_moments8_decode", self.mu.data_ptr(), self.nu.data_ptr(), self.mu_exp.data_ptr(),
-                      self.nu_exp.data_ptr(), self.total, _TYPES[dtype], out[0].data_ptr(), out[1].data_ptr(),
-                      _lib.stream(self.device))
-        return out[0], out[1]
+        mu, nu = (torch.empty(self.total, dtype=dtype, device=self.device) for _ in range(2))
+        self._call("gs_moments8_decode", *self._codes, self.total, _TYPES[dtype], mu.data_ptr(), nu.data_ptr())
+        return mu, nu
 
     def set_values(self, mu: torch.Tensor, nu: torch.Tensor) -> None:
         """Round float32 values in the layout of values() to the nearest codes
-        (values that came from codes are kept exactly; nu >= 0)."""
+        (the values of a block's codes are kept exactly; nu >= 0)."""
         for name, t in (("mu", mu), ("nu", nu)):
             _check_cuda(name, t, (torch.float32,), self.device)
             if t.numel() != self.total:
                 raise ValueError(f"{name}: {t.numel()} values, expected {self.total}")
-        with torch.cuda.device(self.device):
-            _lib.call("gs_moments8_encode", mu.data_ptr(), nu.data_ptr(), self.total, self.mu.data_ptr(),
-                      self.nu.data_ptr(), self.mu_exp.data_ptr(), self.nu_exp.data_ptr(), _lib.stream(self.device))
+        self._call("gs_moments8_encode", mu.data_ptr(), nu.data_ptr(), self.total, *self._codes)
 
     def split(self, flat: torch.Tensor) -> List[torch.Tensor]:
         """The tensors' parts of a buffer in the layout of values()."""
@@ -228,14 +233,15 @@ class AdamW(_Plan):
     change nothing and are counted in `skipped`. max_grad_norm: clip by the
     global norm (optax.clip_by_global_norm) of the gradients, which step() then
     computes first (`norm`, a GradNorm, with grad_scale as its unscale). seed:
-    of the 8-bit moments' stochastic rounding. count: steps already taken.
+    of the 8-bit moments' stochastic rounding. count: steps already taken, or
+    state: the int32 device tensor [steps taken, 0, steps skipped, 0] to use.
     """
 
     def __init__(self, tensors: Sequence[ParamTensor], b1: float = 0.9, b2: float = 0.999, eps: float = 1e-8,
                  moment_bits: Optional[int] = None,
                  moments: Union[None, Moments8, Sequence[Tuple[torch.Tensor, torch.Tensor]]] = None,
                  grad_scale: Optional[torch.Tensor] = None, max_grad_norm: Optional[float] = None, seed: int = 0,
-                 count: int = 0):
+                 count: int = 0, state: Optional[torch.Tensor] = None):
         self.tensors = list(tensors)
         if not self.tensors:
             raise ValueError("no tensors")
@@ -259,8 +265,14 @@ class AdamW(_Plan):
                            for t in self.tensors]
         self.moments = moments
         self._check(sizes)
-        self._state = torch.zeros(4, dtype=torch.int32, device=self.device)
-        self._state[0] = int(count)
+        if state is None:
+            state = torch.zeros(4, dtype=torch.int32, device=self.device)
+            state[0] = int(count)
+        else:
+            _check_cuda("state", state, (torch.int32,), self.device)
+            if state.numel() != 4:
+                raise ValueError("state: expected four int32")
+        self._state = state
         self.count, self.skipped = self._state[0:1], self._state[2:3]
         self.norm = None
         if max_grad_norm is not None:
@@ -274,7 +286,9 @@ class AdamW(_Plan):
         self._table = (_lib.GsAdamwTensor * len(self.tensors))()
         self._fill()
         self._bumped = self._written()
-        self._owned = [self._state] + [t for t in self._moment_buffers()]
+        self._args = (self._table, len(self._table), ctypes.byref(self._config), _lib.ptr(self.grad_scale),
+                      self._state.data_ptr())
+        self._own(self._state, *self._moment_buffers())
 
     def _moment_buffers(self) -> List[torch.Tensor]:
         m = self.moments
@@ -284,7 +298,7 @@ class AdamW(_Plan):
 
     def _written(self) -> List[torch.Tensor]:
         out = [t.param for t in self.tensors] + [t.copy for t in self.tensors if t.copy is not None]
-        return [t for t in out + self._moment_buffers() if not t.is_inference()]
+        return [t for t in out if not t.is_inference()]
 
     def _check(self, sizes: List[int]) -> None:
         dev = self.device
@@ -359,8 +373,7 @@ class AdamW(_Plan):
         """One step on the gradients as they are."""
         if self.norm is not None:
             self.norm()
-        self._call("gs_adamw_step", self._table, len(self._table), ctypes.byref(self._config),
-                   _lib.ptr(self.grad_scale), self._state.data_ptr())
+        self._call("gs_adamw_step", *self._args)
         # the library writes through raw pointers: tell autograd, as an in-place operation does
         torch.autograd.graph.increment_version(self._bumped)
 

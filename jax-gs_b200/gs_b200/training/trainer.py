@@ -20,7 +20,7 @@ from __future__ import annotations
 
 import ctypes
 import dataclasses
-from typing import Dict, Optional, Tuple
+from typing import Dict, List, Optional, Sequence, Tuple
 
 import torch
 
@@ -28,6 +28,7 @@ from gs_b200 import _lib
 from gs_b200._staging import InputStager
 from gs_b200.core.gaussians import Gaussians
 from gs_b200.renderer.rasterizer import workspace
+from gs_b200.training.optimizer import AdamW, Moments8, ParamTensor
 
 # Scalars appended to the gradient buffer so that they share its all-reduce:
 # [l1, d_ssim, ssim_mean, 8 renderer health counters, the render's device
@@ -41,7 +42,15 @@ _METRIC_KEYS = ("n_interactions", "mean_interactions_per_tile", "max_interaction
 
 @dataclasses.dataclass
 class AdamConfig:
-    """optax.multi_transform of per-group optax.adam (train.py:129-156)."""
+    """optax.multi_transform of per-group optax.adam (train.py:129-156).
+
+    The last four fields have no reference counterpart; with one of them away
+    from its default the step updates through gs_adamw_step
+    (gs_b200.training.optimizer): decoupled weight decay per group [means,
+    scales, quaternions, opacities, sh], a clip by the global norm of the
+    gradient (a step whose gradient is not finite is then skipped, counted in
+    DensityState.skipped), Adam moments in 8 bits (a quarter of the memory),
+    and the seed of their stochastic rounding."""
     means_lr_init: float = 0.00016 * 3.0
     means_lr_end: float = 0.0000016 * 3.0
     transition_steps: int = 30000
@@ -52,11 +61,20 @@ class AdamConfig:
     b1: float = 0.9
     b2: float = 0.999
     eps: float = 1e-8
+    weight_decay: Sequence[float] = (0.0, 0.0, 0.0, 0.0, 0.0)
+    max_grad_norm: Optional[float] = None
+    moment_bits: int = 32
+    moment_seed: int = 0
 
     @classmethod
-    def from_extent(cls, extent: float, num_iterations: int = 30000) -> "AdamConfig":
+    def from_extent(cls, extent: float, num_iterations: int = 30000, **kw) -> "AdamConfig":
         return cls(means_lr_init=0.00016 * extent * 3.0, means_lr_end=0.0000016 * extent * 3.0,
-                   transition_steps=num_iterations)
+                   transition_steps=num_iterations, **kw)
+
+    @property
+    def is_adam(self) -> bool:
+        """Whether the update is the reference's plain Adam."""
+        return self.moment_bits == 32 and self.max_grad_norm is None and not any(self.weight_decay)
 
     def lrs(self, count: int):
         """Learning rates of the update whose optax count before increment is
@@ -103,15 +121,24 @@ def _segments(n: int, k: int):
 
 
 class DensityState:
-    """Static-capacity training state (density.py:9-17) in flat buffers."""
+    """Static-capacity training state (density.py:9-17) in flat buffers. With
+    moment_bits = 8 the Adam moments are the codes of `moments8` (a Moments8
+    over the five groups) and mu, nu are None."""
 
-    def __init__(self, n: int, sh_k: int, device):
+    def __init__(self, n: int, sh_k: int, device, moment_bits: int = 32):
         self.n, self.sh_k, self.device = int(n), int(sh_k), torch.device(device)
         self.segments, self.size = _segments(self.n, self.sh_k)
         f = dict(dtype=torch.float32, device=self.device)
         self.params = torch.zeros(self.size, **f)
-        self.mu = torch.zeros(self.size, **f)
-        self.nu = torch.zeros(self.size, **f)
+        if moment_bits not in (8, 32):
+            raise ValueError("moment_bits must be 8 or 32")
+        self.moment_bits = int(moment_bits)
+        self.mu = self.nu = self.moments8 = None
+        if moment_bits == 8:
+            self.moments8 = Moments8([b - a for a, b in self.segments], self.device)
+        else:
+            self.mu = torch.zeros(self.size, **f)
+            self.nu = torch.zeros(self.size, **f)
         self.grads = torch.zeros(self.size + TAIL, **f)
         self.active_mask = torch.zeros(self.n, dtype=torch.bool, device=self.device)
         self.num_active = 0
@@ -120,8 +147,48 @@ class DensityState:
         self.max_radii = torch.zeros(self.n, **f)
         self.count = 0  # optax step count (host mirror)
         # device [optax count, ticket] read and advanced by gs_adam_step_scheduled
-        self.adam_state = torch.zeros(2, dtype=torch.int32, device=self.device)
+        # and gs_adamw_step; then the steps that one skipped, and 0
+        self.adam_state = torch.zeros(4, dtype=torch.int32, device=self.device)
         self._buffers: Dict = {}
+        self._adamw = None  # (hyperparameters, plan) of the last AdamW update
+
+    @property
+    def skipped(self) -> torch.Tensor:
+        """Steps skipped because the gradient's norm was not finite (AdamConfig.max_grad_norm)."""
+        return self.adam_state[2]
+
+    def moment_buffers(self) -> List[torch.Tensor]:
+        """The buffers that hold both Adam moments."""
+        m = self.moments8
+        return [self.mu, self.nu] if m is None else [m.mu, m.nu, m.mu_exp, m.nu_exp]
+
+    def adamw(self, optimizer: AdamConfig) -> AdamW:
+        """The AdamW plan over the five groups (kept until the hyperparameters
+        change; changed rates are taken over)."""
+        hyper = (optimizer.b1, optimizer.b2, optimizer.eps, optimizer.max_grad_norm, optimizer.moment_seed)
+        lrs, wd = optimizer.lrs(0), [float(w) for w in optimizer.weight_decay]
+        if len(wd) != 5:
+            raise ValueError("weight_decay: one value for each of the five groups")
+        decay = [optimizer.means_lr_end / optimizer.means_lr_init, 1.0, 1.0, 1.0, 1.0]
+        rates = list(zip(lrs, wd, decay, [float(optimizer.transition_steps)] + [1.0] * 4))
+        if self._adamw is None or self._adamw[0] != hyper:
+            def rows(buf, i):
+                return buf[self.segments[i][0]:self.segments[i][1]].view(self.n, -1)
+            tensors = [ParamTensor(rows(self.params, i), rows(self.grads, i), *rates[i], active=self.active_mask)
+                       for i in range(5)]
+            moments = self.moments8
+            if moments is None:
+                moments = [(rows(self.mu, i), rows(self.nu, i)) for i in range(5)]
+            plan = AdamW(tensors, b1=optimizer.b1, b2=optimizer.b2, eps=optimizer.eps, moments=moments,
+                         max_grad_norm=optimizer.max_grad_norm, seed=optimizer.moment_seed, state=self.adam_state)
+            self._adamw = [hyper, plan, rates]
+        _, plan, known = self._adamw
+        if known != rates:
+            for t, r in zip(plan.tensors, rates):
+                t.lr, t.weight_decay, t.lr_decay_rate, t.lr_transition_steps = r
+            plan.refresh()
+            self._adamw[2] = rates
+        return plan
 
     def _view(self, buf: torch.Tensor, i: int, shape):
         a, b = self.segments[i]
@@ -175,10 +242,9 @@ class DensityState:
 def init_density_state(gaussians: Gaussians, optimizer: AdamConfig, max_gaussians: int) -> DensityState:
     """Pad to the static capacity (density.py:19-61): padded quaternions are
     identity, everything else zero; active_mask marks the first n_init."""
-    del optimizer
     n0 = int(gaussians.means.shape[0])
     k = int(gaussians.sh_coeffs.shape[1])
-    st = DensityState(max_gaussians, k, gaussians.means.device)
+    st = DensityState(max_gaussians, k, gaussians.means.device, getattr(optimizer, "moment_bits", 32))
     g = st.gaussians
     g.means[:n0] = gaussians.means
     g.scales[:n0] = gaussians.scales
@@ -200,6 +266,11 @@ def _dev_tensor(x, like: torch.Tensor) -> torch.Tensor:
 def _step(state: DensityState, target_image, w2c, camera_static, optimizer: AdamConfig,
           sh_degree: int, group, capacity: Optional[int], lambda_ssim: float = 0.2,
           fused: bool = True):
+    if optimizer.moment_bits != state.moment_bits:
+        raise ValueError(f"the state's moments have {state.moment_bits} bits, the optimizer's {optimizer.moment_bits}")
+    if group is not None and fused and not optimizer.is_adam:
+        raise ValueError("the fused data-parallel update is plain Adam with 32-bit moments: use fused=False with "
+                         "weight decay, max_grad_norm or 8-bit moments")
     W, H, fx, fy, cx, cy = camera_static
     W, H = int(W), int(H)
     fx, fy, cx, cy = float(fx), float(fy), float(cx), float(cy)
@@ -263,10 +334,7 @@ def _step(state: DensityState, target_image, w2c, camera_static, optimizer: Adam
         # statistics (trainer.py:143-159) in one kernel, then Adam
         _lib.call("gs_density_step_stats", P(gf.means), P(p.means), P(w2c_d), n, fx, fy, W, H, P(radii), P(valid),
                   P(mask), P(state.grad_accum), P(state.denom), P(state.max_radii), None, st)
-        state.count += 1
-        sched = optimizer.schedule()
-        _lib.call("gs_adam_step_scheduled", P(state.params), P(state.grads), P(state.mu), P(state.nu), n,
-                  k, P(mask), ctypes.byref(sched), P(state.adam_state), st)
+        _update(state, optimizer, mask, st)
         return b
     pmean_gradients(state.grads, tail, b["extras"], group)
     # grad_2d_mag from the averaged means gradient and pre-update means
@@ -274,15 +342,25 @@ def _step(state: DensityState, target_image, w2c, camera_static, optimizer: Adam
     radii, radii_valid = pmean_grad2d_pmax_radii(b["g2d"], radii, valid, group)
     # Adam + masking + apply (trainer.py:73-77 / 139-141); the schedule is
     # evaluated on the device from state.adam_state so a graph can replay it
-    state.count += 1
-    sched = optimizer.schedule()
-    _lib.call("gs_adam_step_scheduled", P(state.params), P(state.grads), P(state.mu), P(state.nu), n,
-              k, P(mask), ctypes.byref(sched), P(state.adam_state), st)
+    _update(state, optimizer, mask, st)
     # densification statistics (trainer.py:100-113 / 152-159)
     # denom counts this rank's own visibility; max_radii uses the max over ranks
     _lib.call("gs_accumulate_density_stats", P(b["g2d"]), P(radii), P(valid), P(radii_valid), P(mask),
               n, P(state.grad_accum), P(state.denom), P(state.max_radii), st)
     return b
+
+
+def _update(state: DensityState, optimizer: AdamConfig, mask: torch.Tensor, st: int) -> None:
+    """The update from the gradients in state.grads (trainer.py:73-77 /
+    139-141): plain Adam, or AdamW where the optimizer asks for more."""
+    state.count += 1
+    if not optimizer.is_adam:
+        state.adamw(optimizer).step()
+        return
+    P = _lib.ptr
+    sched = optimizer.schedule()
+    _lib.call("gs_adam_step_scheduled", P(state.params), P(state.grads), P(state.mu), P(state.nu), state.n,
+              state.sh_k, P(mask), ctypes.byref(sched), P(state.adam_state), st)
 
 
 def pmean_gradients(grads: torch.Tensor, tail: torch.Tensor, extras: torch.Tensor, group) -> None:
@@ -537,6 +615,7 @@ class CapturedStep:
                   fused=fused)
             self.loss, self.metrics = _loss_metrics(state, b, group, fused)
         self.state.count -= 1  # the capture did not run the step
+        self._plan = state._adamw[1] if state._adamw else None  # the graph holds its buffers' addresses
         self._stager = InputStager(state.device)  # host inputs upload during the previous step
 
     def __call__(self, target_image, w2c):

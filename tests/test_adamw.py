@@ -153,3 +153,29 @@ def test_every_code_keeps_its_value(signed):
         for u in (0.0, 0.5, 0.999):
             c, e = R.encode(x, np.full(256, u), signed)
             np.testing.assert_array_equal(R.decode(c, e, signed), val)
+
+
+def test_trainer_refusals():
+    """The fused data-parallel update is plain Adam; a state and an optimizer
+    agree on the moments' bits; 8-bit moments live on a GPU."""
+    from gs_b200.training import density, trainer
+    st = trainer.DensityState(4, 1, "cpu")
+    cam = (16, 16, 10.0, 10.0, 8.0, 8.0)
+    for kw in (dict(weight_decay=(0.0, 0.1, 0.0, 0.0, 0.0)), dict(max_grad_norm=1.0)):
+        opt = trainer.AdamConfig(**kw)
+        assert not opt.is_adam
+        with pytest.raises(ValueError, match="fused=False"):
+            trainer._step(st, None, None, cam, opt, 0, object(), None)
+    with pytest.raises(ValueError, match="bits"):
+        trainer._step(st, None, None, cam, trainer.AdamConfig(moment_bits=8), 0, None, None)
+    assert trainer.AdamConfig().is_adam and trainer.AdamConfig.from_extent(2.0, max_grad_norm=1.0).max_grad_norm == 1.0
+    with pytest.raises(ValueError, match="CUDA"):
+        trainer.DensityState(4, 1, "cpu", moment_bits=8)
+    with pytest.raises(ValueError, match="moment_bits"):
+        trainer.DensityState(4, 1, "cpu", moment_bits=16)
+    with pytest.raises(ValueError, match="five"):
+        st.adamw(trainer.AdamConfig(weight_decay=(0.1,)))
+    assert [t.data_ptr() for t in st.moment_buffers()] == [st.mu.data_ptr(), st.nu.data_ptr()]
+    st.moments8 = object()
+    with pytest.raises(ValueError, match="8-bit"):
+        density.gather_moments(st, None)
