@@ -247,6 +247,19 @@ __device__ __forceinline__ unsigned any_bits4(const float x[4]) {
   return __float_as_uint(x[0]) | __float_as_uint(x[1]) | __float_as_uint(x[2]) | __float_as_uint(x[3]);
 }
 
+// The two 16-bit values of a word.
+template <int GT>
+__device__ __forceinline__ void two_floats(unsigned w, float& lo, float& hi) {
+  if (GT == GS_TYPE_BF16) {
+    lo = __uint_as_float(w << 16);
+    hi = __uint_as_float(w & 0xFFFF0000u);
+  } else {
+    const float2 t = __half22float2(*reinterpret_cast<const __half2*>(&w));
+    lo = t.x;
+    hi = t.y;
+  }
+}
+
 // Four gradients as loaded (16-bit ones two to a register where VEC).
 template <int GT, bool VEC>
 struct Grad4 {
@@ -266,27 +279,38 @@ struct Grad4 {
       for (int q = 0; q < 4; ++q) w[q] = static_cast<const uint16_t*>(g)[i + 32 * q];
     }
   }
-  __device__ __forceinline__ float get(int q) const {
-    if (GT == GS_TYPE_F32) return __uint_as_float(w[q]);
-    const unsigned h = VEC ? (q & 1 ? w[q >> 1] >> 16 : w[q >> 1] & 0xFFFFu) : w[q];
-    if (GT == GS_TYPE_BF16) return __uint_as_float(h << 16);
-    return __half2float(__ushort_as_half((unsigned short)h));
+  __device__ __forceinline__ void get(float g[4]) const {
+    if (GT == GS_TYPE_F32) {
+#pragma unroll
+      for (int q = 0; q < 4; ++q) g[q] = __uint_as_float(w[q]);
+    } else {
+      two_floats<GT>(VEC ? w[0] : w[0] | w[1] << 16, g[0], g[1]);
+      two_floats<GT>(VEC ? w[1] : w[2] | w[3] << 16, g[2], g[3]);
+    }
   }
 };
 
+// Two floats rounded to the 16-bit type, the first in the low half.
+__device__ __forceinline__ unsigned round2(int type, float lo, float hi) {
+  if (type == GS_TYPE_BF16) {
+    const __nv_bfloat162 t = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const unsigned*>(&t);
+  }
+  const __half2 t = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const unsigned*>(&t);
+}
+
 template <bool VEC>
 __device__ __forceinline__ void store_copy4(void* p, unsigned i, int type, const float x[4]) {
-  unsigned h[4];
-#pragma unroll
-  for (int q = 0; q < 4; ++q)
-    h[q] = type == GS_TYPE_BF16 ? __bfloat16_as_ushort(__float2bfloat16_rn(x[q]))
-                                : __half_as_ushort(__float2half_rn(x[q]));
-  uint16_t* c = static_cast<uint16_t*>(p);
+  const unsigned a = round2(type, x[0], x[1]), b = round2(type, x[2], x[3]);
+  uint16_t* c = static_cast<uint16_t*>(p) + i;
   if (VEC) {
-    *reinterpret_cast<uint2*>(c + i) = make_uint2(h[0] | (h[1] << 16), h[2] | (h[3] << 16));
+    *reinterpret_cast<uint2*>(c) = make_uint2(a, b);
   } else {
-#pragma unroll
-    for (int q = 0; q < 4; ++q) c[i + 32 * q] = (uint16_t)h[q];
+    c[0] = (uint16_t)a;
+    c[32] = (uint16_t)(a >> 16);
+    c[64] = (uint16_t)b;
+    c[96] = (uint16_t)(b >> 16);
   }
 }
 
@@ -435,10 +459,11 @@ __device__ __forceinline__ void adamw32_chunk(const AdamwDesc& d, long long base
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     const unsigned i = i0 + u * kAdamwBlock;
-    float m1[4], v1[4], p1[4];
+    float g1[4], m1[4], v1[4], p1[4];
+    g[u].get(g1);
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
-      const float gq = g[u].get(q) * s;
+      const float gq = g1[q] * s;
       m1[q] = add_rn(mul_rn(m[u][q], a.b1), mul_rn(gq, a.omb1));
       v1[q] = add_rn(mul_rn(v[u][q], a.b2), mul_rn(mul_rn(gq, gq), a.omb2));
     }
@@ -751,12 +776,13 @@ __device__ __forceinline__ int chunk_rows(const AdamwDesc& d, const RowPlace& at
   return __all_sync(0xffffffffu, all) ? kAll : (__any_sync(0xffffffffu, any) ? kSome : kNone);
 }
 
+template <bool LOOSE>
 __device__ __forceinline__ void adamw8_issue(const AdamwDesc& d, Adamw8Chunk& c, Adamw8Stage& st, int lane) {
   const int chunk = (threadIdx.x >> 5) * kChunk8;
   c.kind = kDirect;
   if (d.vec != kScalar && d.count - c.tile >= chunk + kChunk8) {
     const int two = d.grad_type == GS_TYPE_F32 ? 2 : 1;
-    if (d.vec == kVec) {
+    if (!LOOSE || d.vec == kVec) {
       const char* g = static_cast<const char*>(d.grad) + (c.tile << two) + (unsigned)((chunk << two) + 16 * lane);
       char* sg = reinterpret_cast<char*>(st.g) + 16 * lane;
       cp_async16(sg, g);
@@ -787,7 +813,7 @@ __device__ __forceinline__ void adamw8_issue(const AdamwDesc& d, Adamw8Chunk& c,
     }
     if (c.kind != kNone || d.copy) {
       const float* p = d.param + c.tile + (unsigned)chunk;
-      if (d.vec == kVec) {
+      if (!LOOSE || d.vec == kVec) {
 #pragma unroll
         for (int n = 0; n < 4; ++n) cp_async16(st.p + 4 * lane + 128 * n, p + 4 * lane + 128 * n);
       } else {
@@ -805,10 +831,8 @@ __device__ __forceinline__ void grads4(const unsigned* st, int e, float g[4]) {
     load4<true>(reinterpret_cast<const float*>(st), e, g);
   } else {
     const uint2 w = *reinterpret_cast<const uint2*>(reinterpret_cast<const uint16_t*>(st) + e);
-    const unsigned x[4] = {w.x << 16, w.x & 0xFFFF0000u, w.y << 16, w.y & 0xFFFF0000u};
-#pragma unroll
-    for (int q = 0; q < 4; ++q)
-      g[q] = GT == GS_TYPE_BF16 ? __uint_as_float(x[q]) : __half2float(__ushort_as_half((unsigned short)(x[q] >> 16)));
+    two_floats<GT>(w.x, g[0], g[1]);
+    two_floats<GT>(w.y, g[2], g[3]);
   }
 }
 
@@ -914,7 +938,7 @@ __device__ __forceinline__ void adamw8_chunk(const AdamwDesc& d, const Adamw8Chu
     }
     if (__all_sync(0xffffffffu, any == 0u)) return;
   }
-#pragma unroll
+#pragma unroll 1
   for (int j = 0; j < 2; ++j) adamw8_blocks<GT, ALL, COPY, LOOSE>(d, c, st, j, exps, a, h, s, key, lane);
   if (lane < 8)
     ((lane < 4 ? d.mu_exp : d.nu_exp) + c.tile / kAdamwBlock)[(threadIdx.x >> 5) * 4 + (lane & 3)] = (uint8_t)exps;
@@ -938,7 +962,9 @@ __device__ __forceinline__ void adamw8_typed(const AdamwDesc& d, const Adamw8Chu
   }
 }
 
-template <int N>
+// LOOSE: tensors with kLoose are among the table's (a kernel of its own: the
+// code for them costs the others 3 %).
+template <int N, bool LOOSE>
 __global__ void __launch_bounds__(32 * kWarps8, GS_ADAMW8_CTAS)
 k_adamw8(const __grid_constant__ AdamwTable<N> tab, const __grid_constant__ AdamwParams a) {
   GS_PDL_ENTRY_PLAIN();
@@ -952,7 +978,7 @@ k_adamw8(const __grid_constant__ AdamwTable<N> tab, const __grid_constant__ Adam
   if (more) {
     now.k = w.k;
     now.tile = w.base();
-    adamw8_issue(tab.t[now.k], now, st[0], lane);
+    adamw8_issue<LOOSE>(tab.t[now.k], now, st[0], lane);
   }
   const unsigned ticket = adamw_head(a, head);
   if (head.go) {
@@ -968,7 +994,7 @@ k_adamw8(const __grid_constant__ AdamwTable<N> tab, const __grid_constant__ Adam
       if (more) {
         next.k = w.k;
         next.tile = w.base();
-        adamw8_issue(tab.t[next.k], next, st[at ^ 1], lane);
+        adamw8_issue<LOOSE>(tab.t[next.k], next, st[at ^ 1], lane);
         asm volatile("cp.async.wait_group 1;" ::: "memory");
       } else {
         asm volatile("cp.async.wait_group 0;" ::: "memory");
@@ -981,7 +1007,7 @@ k_adamw8(const __grid_constant__ AdamwTable<N> tab, const __grid_constant__ Adam
         last = now.k;
       }
       if (now.kind != kDirect) {
-        if (d.vec == kLoose) adamw8_typed<GS_TYPE_F32, true>(d, now, st[at], a, h, s, tkey, lane);
+        if (LOOSE && d.vec == kLoose) adamw8_typed<GS_TYPE_F32, true>(d, now, st[at], a, h, s, tkey, lane);
         else if (d.grad_type == GS_TYPE_F32) adamw8_typed<GS_TYPE_F32, false>(d, now, st[at], a, h, s, tkey, lane);
         else if (d.grad_type == GS_TYPE_BF16) adamw8_typed<GS_TYPE_BF16, false>(d, now, st[at], a, h, s, tkey, lane);
         else adamw8_typed<GS_TYPE_F16, false>(d, now, st[at], a, h, s, tkey, lane);
@@ -1066,12 +1092,14 @@ static void launch_adamw_class(const GsAdamwTensor* t, int n, int index0, const 
   const bool small = blocks <= (long long)device_sms() * GS_ADAMW_SMALL;
   const int tile = small ? kSmallWarps * kAdamwBlock : kAdamwTile;
   int tiles = 0, entries = 0;
+  bool loose = false;
   for (int i = 0; i < n; ++i) {
     AdamwDesc d[2];
     const int k = describe(t[i], index0 + i, BITS, d);
     if (small && k == 2) d[0].count = t[i].count;  // element by element all the same
     for (int j = 0; j < (small ? 1 : k); ++j) {
       tab.t[entries] = d[j];
+      loose |= d[j].vec == kLoose;
       tab.first[entries++] = tiles;
       tiles += (int)((d[j].count + tile - 1) / tile);
     }
@@ -1082,7 +1110,8 @@ static void launch_adamw_class(const GsAdamwTensor* t, int n, int index0, const 
   if (small) {
     launch_kernel_plain(k_adamw_small<BITS, N>, std::max(1, tiles), 32 * kSmallWarps, 0, st, tab, a);
   } else if (BITS == 8) {
-    launch_kernel_plain(k_adamw8<N>, std::min(tiles, device_sms() * GS_ADAMW8_CTAS), 32 * kWarps8, 0, st, tab, a);
+    launch_kernel_plain(loose ? k_adamw8<N, true> : k_adamw8<N, false>, std::min(tiles, device_sms() * GS_ADAMW8_CTAS),
+                        32 * kWarps8, 0, st, tab, a);
   } else {
     launch_kernel_plain(k_adamw32<N>, std::min(tiles, device_sms() * 8), 32 * kAdamwWarps, 0, st, tab, a);
   }
@@ -1167,13 +1196,7 @@ __device__ __forceinline__ void norm_add(const uint4& w, double acc[4]) {
       acc[q] = fma(x, x, acc[q]);
     } else {
       float lo, hi;
-      if (GT == GS_TYPE_BF16) {
-        lo = __uint_as_float(b[q] << 16);
-        hi = __uint_as_float(b[q] & 0xFFFF0000u);
-      } else {
-        lo = __half2float(__ushort_as_half((unsigned short)(b[q] & 0xFFFFu)));
-        hi = __half2float(__ushort_as_half((unsigned short)(b[q] >> 16)));
-      }
+      two_floats<GT>(b[q], lo, hi);
       const double x = (double)lo, y = (double)hi;
       acc[q] = fma(x, x, acc[q]);
       acc[q] = fma(y, y, acc[q]);
