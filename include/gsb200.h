@@ -590,7 +590,8 @@ typedef struct GsAdamwConfig {
  * all of which reads as NaN. The step rounds up or down at random, with the
  * probabilities that keep the mean, from 16 bits of a hash of (seed, c,
  * index of the tensor, block, element) for each moment; nu' > 0 never becomes
- * 0. The parameter's update uses the new moments before they are rounded.
+ * 0. The sign of a zero mu is not specified. The parameter's update uses the
+ * new moments before they are rounded.
  */
 GS_API int gs_adamw_step(const GsAdamwTensor* tensors, int n_tensors, const GsAdamwConfig* config,
                          const float* grad_scale, int32_t* state, gs_stream_t stream);
@@ -598,7 +599,7 @@ GS_API int gs_adamw_step(const GsAdamwTensor* tensors, int n_tensors, const GsAd
 /*
  * Global norm of a gradient (optax.global_norm) and the factor that clips it
  * (optax.clip_by_global_norm): over all elements of all tensors,
- *   norm  = u sqrt(sum grad^2),  u = *unscale (1 if NULL), e.g. 1 / loss scale
+ *   norm  = u sqrt(sum grad^2),  u = *unscale > 0 (1 if NULL), e.g. 1 / loss scale
  *   scale = u * (norm < max_norm ? 1 : max_norm / norm)
  * scale is NaN when the norm is not finite (in fp32). &out->scale is a
  * grad_scale for gs_adamw_step, which then clips, or skips the step, without

@@ -8,7 +8,7 @@
 //   p' = p - lr (m' / (1 - b1^t) / (sqrt(v' / (1 - b2^t)) + eps) + wd p)
 // in fp32 throughout; m' and v' are sums of two rounded products (no FMA), so
 // that the 8-bit codes are a function of the inputs that any fp32
-// implementation reproduces bit for bit. p' needs no such care: its divide
+// implementation reproduces bit for bit (but the sign of a zero). p' needs no such care: its divide
 // and square root are the approximate ones (a few ulps of the update).
 //
 // 8-bit moments. A block is 128 elements from the tensor's start: one warp,
@@ -927,12 +927,17 @@ __device__ __forceinline__ void adamw8_chunk(const AdamwDesc& d, const Adamw8Chu
                                              const AdamwParams& a, const AdamwStep& h, float s, unsigned key, int lane) {
   unsigned exps = 0u;
   if (!ALL && !COPY && c.kind == kNone) {
-    // moments and gradients all zero in rows that are not active: nothing changes
+    // moments and gradients all zero in rows that are not active: nothing
+    // changes but for the sign of a zero. (An exponent byte of 0 alone may be
+    // a block of subnormals.)
     unsigned any = lane < 8 ? c.exps : 0u;
 #pragma unroll
     for (int n = 0; n < 4; ++n) {
+      const int e = group8(n >> 1, n & 1, lane);
+      any |= (*reinterpret_cast<const unsigned*>(st.mu + e) & 0x7F7F7F7Fu) |
+             *reinterpret_cast<const unsigned*>(st.nu + e);
       float g[4];
-      grads4<GT>(st.g, group8(n >> 1, n & 1, lane), g);
+      grads4<GT>(st.g, e, g);
 #pragma unroll
       for (int q = 0; q < 4; ++q) any |= __float_as_uint(g[q]) << 1;
     }
@@ -1024,10 +1029,28 @@ k_adamw8(const __grid_constant__ AdamwTable<N> tab, const __grid_constant__ Adam
   adamw_finish(a, head, ticket);
 }
 
-// One entry for a tensor, or two: with 32-bit moments a tensor whose arrays
-// all lie the same elements behind a 16-byte boundary (the groups of a flat
-// buffer of odd capacity) is cut after the elements up to the next one, and
-// the rest is accessed four elements at a time.
+// With 32-bit moments, how many elements all arrays of a tensor lie behind a
+// 16-byte boundary (8 bytes for 16-bit values); -1 where they differ.
+static int elements_behind(const GsAdamwTensor& t) {
+  const uintptr_t p = (uintptr_t)t.param, g = (uintptr_t)t.grad, m = (uintptr_t)t.mu, v = (uintptr_t)t.nu,
+                  c = (uintptr_t)t.copy;
+  const uintptr_t behind = p / 4 & 3;
+  const bool same = (m / 4 & 3) == behind && (v / 4 & 3) == behind &&
+                    ((t.grad_type == GS_TYPE_F32 ? g / 4 : g / 2) & 3) == behind &&
+                    (!t.copy || (c / 2 & 3) == behind);
+  return same ? (int)behind : -1;
+}
+
+// Entries of a tensor in the table: one, or two with 32-bit moments where all
+// arrays lie the same 1 to 3 elements behind a boundary (the groups of a flat
+// buffer of odd capacity): the elements up to the next boundary, and the rest,
+// which is accessed four elements at a time (333331 slots: 67 us element by
+// element, 63 us so).
+static int entries_of(const GsAdamwTensor& t, int bits) {
+  const int behind = bits == 32 ? elements_behind(t) : 0;
+  return behind > 0 && t.count > 4 - behind ? 2 : 1;
+}
+
 static int describe(const GsAdamwTensor& t, int index, int bits, AdamwDesc out[2]) {
   AdamwDesc d;
   d.param = t.param;
@@ -1040,7 +1063,7 @@ static int describe(const GsAdamwTensor& t, int index, int bits, AdamwDesc out[2
   d.active = t.active;
   d.count = t.count;
   d.lr_init = t.lr_init;
-  d.ln_decay = (float)(std::log((double)t.decay_rate) / (double)t.transition_steps);
+  d.ln_decay = t.decay_rate == 1.f ? 0.f : (float)(std::log((double)t.decay_rate) / (double)t.transition_steps);
   d.weight_decay = t.weight_decay;
   d.width = (unsigned)t.width;
   d.magic = t.width > 1 ? ~0ull / (unsigned)t.width + 1ull : 0ull;
@@ -1048,27 +1071,20 @@ static int describe(const GsAdamwTensor& t, int index, int bits, AdamwDesc out[2
   d.copy_type = (uint8_t)t.copy_type;
   d.skip = 0;
   d.index = index;
-  const uintptr_t p = (uintptr_t)t.param, g = (uintptr_t)t.grad, m = (uintptr_t)t.mu, v = (uintptr_t)t.nu,
-                  c = (uintptr_t)t.copy;
   const bool f32 = t.grad_type == GS_TYPE_F32;
   d.vec = kScalar;
   if (bits == 8) {
-    if (((m | v) & 15) == 0 && (c & 7) == 0) d.vec = ((p | g) & 15) == 0 ? kVec : (f32 ? kLoose : kScalar);
+    const uintptr_t pg = (uintptr_t)t.param | (uintptr_t)t.grad;
+    if ((((uintptr_t)t.mu | (uintptr_t)t.nu) & 15) == 0 && ((uintptr_t)t.copy & 7) == 0)
+      d.vec = (pg & 15) == 0 ? kVec : (f32 ? kLoose : kScalar);
     out[0] = d;
     return 1;
   }
-  const uintptr_t behind = p / 4 & 3;  // elements behind a boundary
-  const bool same = (m / 4 & 3) == behind && (v / 4 & 3) == behind &&
-                    (f32 ? (g / 4 & 3) == behind : (g & 1) == 0 && (g / 2 & 3) == behind) &&
-                    (!t.copy || (c / 2 & 3) == behind);
+  const int behind = elements_behind(t);
+  if (behind == 0) d.vec = kVec;
   out[0] = d;
-  if (!same) return 1;
-  if (behind == 0) {
-    out[0].vec = kVec;
-    return 1;
-  }
-  const int64_t head = 4 - (int64_t)behind;
-  if (t.count <= head) return 1;
+  if (entries_of(t, bits) == 1) return 1;
+  const int64_t head = 4 - behind;
   out[0].count = head;
   d.param += head;
   d.grad = static_cast<const char*>(d.grad) + head * (f32 ? 4 : 2);
@@ -1125,8 +1141,8 @@ static void launch_adamw_bits(const GsAdamwTensor* tensors, int n, AdamwParams& 
   do {
     // as many tensors as have entries
     int entries = 0, take = 0;
-    for (AdamwDesc d[2]; at + take < n; ++take) {
-      const int k = describe(tensors[at + take], 0, BITS, d);
+    for (; at + take < n; ++take) {
+      const int k = entries_of(tensors[at + take], BITS);
       if (entries + k > kAdamwMost) break;
       entries += k;
     }

@@ -543,3 +543,154 @@ def test_refusals():
         Moments8([8], mu=z(8, torch.uint8), nu=z(128, torch.uint8), mu_exp=z(1, torch.uint8), nu_exp=z(1, torch.uint8))
     with pytest.raises(ValueError, match="dtype"):
         Moments8([8], "cuda").values(torch.float16)
+
+
+# ---- the kernels for many elements (the others above run in the kernel for few) ------------------------------
+
+
+BIG = [700_001, 513, 0, 4097, 2048, 130, 1]
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("grad,copy,align", [
+    ("f32", None, 128), ("f32", "bf16", 128), ("bf16", None, 128), ("bf16", "bf16", 128), ("f16", "f16", 128),
+    ("f16", None, 128), ("f32", None, 1), ("f32", None, 4), ("f32", None, 2), ("f32", "f16", 1), ("bf16", None, 1),
+    ("bf16", "bf16", 1), ("f16", "f16", 4), ("bf16", None, 2)])
+def test_many_elements(bits, grad, copy, align):
+    s = Setup(BIG, bits, grad=grad, copy=copy, align=align, seed=21, grad_scale=torch.tensor(0.7, device="cuda"))
+    for _ in range(2):
+        s.step_and_check(scale=np.float32(0.7))
+    pad = torch.ones_like(s.flat_p, dtype=torch.bool)
+    for p in s.p:
+        a = (p.data_ptr() - s.flat_p.data_ptr()) // 4
+        pad[a:a + p.numel()] = False
+    assert (s.flat_p[pad] == 7.0).all()
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("copy", [None, "bf16"])
+@pytest.mark.parametrize("align", [128, 1])
+def test_many_rows(bits, copy, align):
+    """Masks with whole chunks on, whole chunks off and changing row by row; widths from 1 to the largest."""
+    rng = np.random.default_rng(0)
+    n = 20_011
+    flags = rng.uniform(size=n) < 0.5
+    flags[:9000] = True
+    flags[11_000:] = False
+    mask = torch.tensor(flags, device="cuda")
+    wide = torch.tensor([True, False, True], device="cuda")
+    widths = [3, 1, 4, 48, 7, 32_768]
+    active = [mask] * 5 + [wide]
+    s = Setup([n * w for w in widths[:5]] + [3 * widths[5]], bits, active=active, copy=copy, align=align, seed=22)
+    for g, act, w in zip(s.g, active, widths):  # rows that are off have no gradient, as in a scene
+        g.view(-1, w)[~act] = 0.0
+    for _ in range(2):
+        s.step_and_check()
+
+
+def test_tensors_of_all_kinds_in_one_call():
+    from gs_b200.training.optimizer import AdamW, Moments8, ParamTensor
+    rng = np.random.default_rng(4)
+    sizes = [300_001, 250_000, 100_000, 99_999, 5000]
+    kinds = [("f32", 0, None), ("f32", 1, "bf16"), ("bf16", 0, None), ("f16", 1, "f16"), ("bf16", 3, None)]
+    for bits in (32, 8):
+        tensors = []
+        for n, (grad, off, copy) in zip(sizes, kinds):
+            p = torch.tensor(rng.standard_normal(n + off).astype(np.float32), device="cuda")[off:]
+            g = torch.tensor(rng.standard_normal(n + off).astype(np.float32), device="cuda").to(DT[grad])[off:]
+            c = torch.zeros(n, dtype=DT[copy], device="cuda") if copy else None
+            tensors.append(ParamTensor(p, g, lr=1e-3, weight_decay=0.1, copy=c))
+        opt = AdamW(tensors, moment_bits=bits, seed=3)
+        p0 = [t.param.cpu().numpy() for t in tensors]
+        opt.step()
+        for i, (t, (mu, nu), n) in enumerate(zip(tensors, opt.moment_values(), sizes)):
+            z = np.zeros(n, np.float32)
+            m, v = R.moments(z, z, t.grad.float().cpu().numpy(), 1.0, 0.9, 0.999)
+            want, err = R.param(p0[i], m, v, 0, 1e-3, 0.1, 0.9, 0.999, 1e-8)
+            assert (np.abs(t.param.cpu().numpy() - want) <= err).all(), i
+            if bits == 32:
+                np.testing.assert_array_equal(mu.cpu().numpy(), m)
+                np.testing.assert_array_equal(nu.cpu().numpy(), v)
+            else:
+                h = R.noise(3, 0, i, n)
+                np.testing.assert_array_equal(mu.cpu().numpy(), R.decode(*R.encode(m, (h % 65536) / 65536.0, True), True))
+                np.testing.assert_array_equal(nu.cpu().numpy(),
+                                              R.decode(*R.encode(v, (h // 65536) / 65536.0, False), False))
+            if t.copy is not None:
+                assert torch.equal(t.copy, t.param.to(t.copy.dtype))
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_subnormal_moments_of_rows_that_are_off_decay(bits):
+    """Exponent byte 0 does not mean zero: a block of subnormal moments goes on, whatever the mask."""
+    n = 800_000
+    off = torch.zeros(n, dtype=torch.bool, device="cuda")
+    s = Setup([n], bits, active=[off], seed=23)
+    s.g[0].fill_(0.0)
+    s.g[0].view(-1)[:300_000] = 2e-39 * torch.arange(300_000, device="cuda").remainder(7)
+    s.step_and_check()
+    s.g[0].fill_(0.0)
+    for _ in range(2):
+        s.step_and_check()
+    assert float(s.opt.moment_values()[0][0].abs().max()) > 0
+
+
+def test_extreme_gradients_of_many_elements():
+    s = Setup([655_360], 8, seed=24)
+    rng = np.random.default_rng(1)
+    g = (rng.choice([-1.0, 1.0], 655_360) * 10.0 ** rng.uniform(-44, 18, 655_360)).astype(np.float32)
+    g[:1024] = np.float32(1e18)
+    g[4096:5000] = 0.0
+    s.g[0].copy_(torch.tensor(g))
+    for _ in range(2):
+        s.step_and_check()
+    s.g[0][10_000] = float("nan")
+    s.g[0][20_000] = float("-inf")
+    s.opt.step()
+    mu, nu = (np.isnan(x.cpu().numpy()) for x in s.opt.moments.values())
+    bad = np.zeros(655_360, bool)
+    for e in (10_000, 20_000):
+        bad[e // 128 * 128:e // 128 * 128 + 128] = True
+    np.testing.assert_array_equal(mu, bad)
+    np.testing.assert_array_equal(nu, bad)
+    np.testing.assert_array_equal(np.flatnonzero(np.isnan(s.p[0].cpu().numpy())), [10_000, 20_000])
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_many_elements_skip_and_replay(bits):
+    """A skipped step of the large kernels leaves everything; replays equal eager steps."""
+    scale = torch.tensor(math.nan, device="cuda")
+    s = Setup(BIG, bits, copy="f16", grad_scale=scale)
+    before = s.read()
+    s.opt.step()
+    for x, y in zip(before, s.read()):
+        for a, b in zip(x, y):
+            np.testing.assert_array_equal(a, b)
+    assert int(s.opt.count) == 0 and int(s.opt.skipped) == 1
+    scale.fill_(1.0)
+    t = Setup(BIG, bits, copy="f16")
+    graph = torch.cuda.CUDAGraph()
+    s.opt.step()
+    t.opt.step()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        t.opt.step()
+    for _ in range(2):
+        s.opt.step()
+        graph.replay()
+    for x, y in zip(s.read(), t.read()):
+        for a, b in zip(x, y):
+            np.testing.assert_array_equal(a, b)
+    assert int(t.opt.count) == 3
+
+
+def test_no_tensors_is_a_step():
+    import ctypes
+    from gs_b200 import _lib
+    state = torch.zeros(4, dtype=torch.int32, device="cuda")
+    cfg = _lib.GsAdamwConfig(b1=0.9, b2=0.999, eps=1e-8, moment_bits=8, seed=0)
+    out = torch.zeros(4, device="cuda")
+    ws = torch.empty(_lib.lib().gs_grad_norm_workspace_bytes(0), dtype=torch.uint8, device="cuda")
+    _lib.call("gs_adamw_step", None, 0, ctypes.byref(cfg), None, _lib.ptr(state), _lib.stream(state.device))
+    _lib.call("gs_grad_norm", None, 0, 1.0, None, _lib.ptr(out), _lib.ptr(ws), ws.numel(), _lib.stream(state.device))
+    assert state.tolist() == [1, 0, 0, 0] and out[:2].tolist() == [0.0, 1.0]
