@@ -243,6 +243,12 @@ __device__ __forceinline__ void store4(float* p, unsigned i, const float x[4]) {
   }
 }
 
+__device__ __forceinline__ unsigned differ4(const float x[4], const float y[4]) {
+  unsigned d = 0u;
+#pragma unroll
+  for (int q = 0; q < 4; ++q) d |= __float_as_uint(x[q]) ^ __float_as_uint(y[q]);
+  return d;
+}
 __device__ __forceinline__ unsigned any_bits4(const float x[4]) {
   return __float_as_uint(x[0]) | __float_as_uint(x[1]) | __float_as_uint(x[2]) | __float_as_uint(x[3]);
 }
@@ -476,7 +482,7 @@ __device__ __forceinline__ void adamw32_chunk(const AdamwDesc& d, long long base
     // the parameters of rows that are not active, and moments that were and
     // stay zero (slots that never had a gradient), are not stored again
     if (bits != 0u) store4<VEC>(param, i, p1);
-    if (any_bits4(m1) | any_bits4(v1) | any_bits4(m[u]) | any_bits4(v[u])) {
+    if (differ4(m1, m[u]) | differ4(v1, v[u]) | ((any_bits4(m[u]) | any_bits4(v[u])) << 1)) {
       store4<VEC>(mu, i, m1);
       store4<VEC>(nu, i, v1);
     }
