@@ -11,8 +11,8 @@
 // implementation reproduces bit for bit (but the sign of a zero). p' needs no such care: its divide
 // and square root are the approximate ones (a few ulps of the update).
 //
-// 8-bit moments. A block is 128 elements from the tensor's start: one warp,
-// four elements a lane. Each moment has one exponent byte a block,
+// 8-bit moments. A block is 128 elements, counted from the tensor's start.
+// Each moment has one exponent byte a block,
 //   F = (bits(max |x|) + 0xfffff) >> 23,
 // the smallest biased power of two under which the maximum, rounded up to 3
 // mantissa bits, still has the top code. Scaling by a power of two is exact,
@@ -28,8 +28,13 @@
 // nonzero m over sqrt(0) + eps would be unbounded). F = 255 marks a block
 // with a value that is not finite: all of it reads as NaN.
 //
-// The kernels are bound by HBM: 28 B an element with 32-bit moments and fp32
-// gradients, 16 B with 8-bit ones.
+// Bytes an element with fp32 gradients: 28 with 32-bit moments, 16 with 8-bit
+// ones. Measured on a B200 whose copies run at 6.45 TB/s: the 32-bit step on
+// 59M elements 260 us (28 B: 6.35 TB/s, bound by HBM); the 8-bit step on 236M
+// elements, a quarter of them in rows that are off, 572 us (13.5 B moved:
+// 5.6 TB/s), bound by HBM and by the issue of 62 instructions an element
+// (2.7 of 4 a cycle); the norm of 236M fp32 gradients 141 us (6.7 TB/s, some
+// of it from L2).
 #include <algorithm>
 #include <cmath>
 
@@ -40,29 +45,43 @@
 
 namespace gs {
 
-constexpr int kAdamwBlock = GS_ADAMW_BLOCK;  // elements of a quantisation block and of a warp's unit of work
+constexpr int kAdamwBlock = GS_ADAMW_BLOCK;  // elements of a block of 8-bit moments, and what a warp does at least
 constexpr int kAdamwWarps = 8;
-constexpr int kAdamwUnroll = 2;  // blocks of a chunk, what a warp takes at a time
+constexpr int kAdamwUnroll = 2;  // blocks of a chunk, what a warp takes at a time (32-bit moments)
 constexpr int kAdamwChunk = kAdamwBlock * kAdamwUnroll;
 constexpr int kAdamwTile = kAdamwChunk * kAdamwWarps;  // elements a CTA takes at a time
 static_assert(kAdamwBlock == 128, "a warp holds a block, four elements a lane");
+// CTAs an SM, which bound the registers. 32-bit moments, 59M elements: 2 or 3
+// CTAs of 256 262 us, 4 276, 5 291 (and 1 block a chunk 278, 4 blocks 264).
+#ifndef GS_ADAMW_CTAS
+#define GS_ADAMW_CTAS 3
+#endif
+// 8-bit moments, 236M elements: 5 CTAs of 128 (as many as the shared memory
+// holds) 567 us, 4 596.
+#ifndef GS_ADAMW8_CTAS
+#define GS_ADAMW8_CTAS 5
+#endif
+// Blocks per SM up to which every warp takes one (k_adamw_small). 32-bit
+// moments: 118k elements 4.3 us so and 4.6 in chunks, 177k 4.4 and 4.0, 590k
+// 5.5 and 4.3. 8-bit: 59k 4.8 and 7.1, 590k 6.9 and 7.4, 885k 8.2 and 7.5.
 #ifndef GS_ADAMW_SMALL
-#define GS_ADAMW_SMALL 32
+#define GS_ADAMW_SMALL 8
 #endif
-#ifndef GS_DECODE_UNROLL
-#define GS_DECODE_UNROLL 2
+#ifndef GS_ADAMW8_SMALL
+#define GS_ADAMW8_SMALL 32
 #endif
+// Gradient norm: 16-byte loads a thread has in flight, and CTAs of 256 an SM.
+// 236M fp32 gradients: 2 x 8 and 4 x 4 141 us (the rate of a copy), 2 x 4 173.
 #ifndef GS_NORM_VECS
 #define GS_NORM_VECS 2
 #endif
 #ifndef GS_NORM_CTAS
 #define GS_NORM_CTAS 8
 #endif
-#ifndef GS_ADAMW_CTAS
-#define GS_ADAMW_CTAS 3
-#endif
-#ifndef GS_ADAMW8_CTAS
-#define GS_ADAMW8_CTAS 5
+// Decoding: groups of 8 codes of each moment a thread has in flight. 236M
+// elements to bf16: 1 252 us, 2 244, 4 251.
+#ifndef GS_DECODE_UNROLL
+#define GS_DECODE_UNROLL 2
 #endif
 
 // One tensor as the kernels see it.
@@ -83,8 +102,10 @@ struct AdamwDesc {
   uint8_t skip;  // elements of the first row that lie before the first element (below 4)
   int index;     // place in the caller's list (the noise key)
 };
-// AdamwDesc::vec: accesses of four elements, of one, and (8-bit moments) of
-// four but for a parameter and fp32 gradient that are not 16-byte aligned.
+// AdamwDesc::vec: accesses of one element, of four, and (8-bit moments, fp32
+// gradients) of four but for the parameter and the gradient, which are not
+// 16-byte aligned: they pass through shared memory word by word (59M elements:
+// 200 us, aligned 160).
 constexpr int kScalar = 0, kVec = 1, kLoose = 2;
 
 // Tables travel as kernel parameters (no device copy, nothing to keep alive,
@@ -97,8 +118,7 @@ struct AdamwTable {
 };
 
 // The tensor of a tile, the last whose first tile is not behind it, by a whole
-// warp: 32 entries at a time (one after the other, 200 tensors' entries took
-// longer to read than their tiles). first[n] is behind every tile.
+// warp, 32 entries at a time. first[n] is behind every tile.
 template <int N>
 __device__ __forceinline__ int tensor_after(const int (&first)[N], int n, int tile, int k) {
   const int lane = threadIdx.x & 31;
@@ -220,8 +240,7 @@ __device__ __forceinline__ int block_element(int lane, int q) {
   return VEC ? 4 * lane + q : lane + 32 * q;
 }
 
-// Accesses are a pointer that is the same in all threads plus a 32-bit
-// element offset `i` of the lane's first element.
+// Four elements of a lane, the first at p[i].
 template <bool VEC>
 __device__ __forceinline__ void load4(const float* p, unsigned i, float x[4]) {
   if (VEC) {
@@ -491,7 +510,7 @@ __device__ __forceinline__ void adamw32_chunk(const AdamwDesc& d, long long base
 
 // Up to one block by one warp, `rem` elements of it in range, element by
 // element: the ends of tensors, few elements in all, and, with 8-bit moments,
-// tensors whose pointers are not 16-byte aligned.
+// tensors that are kScalar.
 template <int BITS>
 struct AdamwBlock {
   long long base;
@@ -588,14 +607,16 @@ struct AdamwBlock {
   }
 };
 
-// A tile's elements behind its `full` whole chunks (those of the first warps),
-// block by block, by the other warps.
-template <int BITS>
-__device__ __forceinline__ void adamw_blocks(const AdamwDesc& d, long long tile, int full, int warps, int chunk,
-                                             const AdamwParams& a, const AdamwStep& h, float s, unsigned key) {
-  const int end = (int)min(d.count - tile, (long long)kAdamwTile), warp = threadIdx.x >> 5;
+// A tile's elements behind its `full` whole chunks, which are the first
+// warps', block by block, the warps without a chunk first.
+template <int BITS, int WARPS>
+__device__ __forceinline__ void adamw_blocks(const AdamwDesc& d, long long tile, int full, const AdamwParams& a,
+                                             const AdamwStep& h, float s, unsigned key) {
+  static_assert((WARPS & (WARPS - 1)) == 0, "");
+  const int end = (int)min(d.count - tile, (long long)kAdamwTile);
+  int e = full * (kAdamwTile / WARPS) + (((int)(threadIdx.x >> 5) - full) & (WARPS - 1)) * kAdamwBlock;
 #pragma unroll 1
-  for (int e = full * chunk + (warp - full) * kAdamwBlock; e < end; e += (warps - full) * kAdamwBlock) {
+  for (; e < end; e += WARPS * kAdamwBlock) {
     AdamwBlock<BITS> b;
     b.load(d, tile + e, min(end - e, kAdamwBlock));
     b.step(d, a, h, s, key);
@@ -680,9 +701,8 @@ k_adamw32(const __grid_constant__ AdamwTable<N> tab, const __grid_constant__ Ada
       const AdamwDesc& d = tab.t[w.k];
       if (w.k != last) adamw_rates(h, d, cf);
       last = w.k;
-      const int full = (int)min((d.count - w.base()) / kAdamwChunk, (long long)kAdamwWarps);
-      if ((int)(threadIdx.x >> 5) < full) {
-        const long long base = w.base() + (threadIdx.x >> 5) * kAdamwChunk;
+      const long long base = w.base() + (threadIdx.x >> 5) * kAdamwChunk;
+      if (d.count - base >= kAdamwChunk) {
         switch (d.grad_type * 2 + (d.vec == kVec)) {
           case 0: adamw32_chunk<GS_TYPE_F32, false>(d, base, a, h, s); break;
           case 1: adamw32_chunk<GS_TYPE_F32, true>(d, base, a, h, s); break;
@@ -691,8 +711,10 @@ k_adamw32(const __grid_constant__ AdamwTable<N> tab, const __grid_constant__ Ada
           case 4: adamw32_chunk<GS_TYPE_F16, false>(d, base, a, h, s); break;
           default: adamw32_chunk<GS_TYPE_F16, true>(d, base, a, h, s); break;
         }
-      } else {
-        adamw_blocks<32>(d, w.base(), full, kAdamwWarps, kAdamwChunk, a, h, s, 0u);
+      }
+      if (d.count - w.base() < kAdamwTile) {
+        // what is left of the tensor behind its chunks, at most a block a warp
+        adamw_blocks<32, kAdamwWarps>(d, w.base(), (int)(d.count - w.base()) / kAdamwChunk, a, h, s, 0u);
       }
     }
   }
@@ -728,7 +750,8 @@ k_adamw_small(const __grid_constant__ AdamwTable<N> tab, const __grid_constant__
 }
 
 // 8-bit moments. The step's instructions take the SMs about as long as its
-// bytes take the memory, so
+// bytes take the memory (the same step with a block a warp and every test at
+// each element: 98 instructions, 765 us at 236M elements, now 62 and 572), so
 //  - no warp waits for memory: each copies its next chunk into shared memory
 //    (cp.async, 16 bytes a lane) before it works on the current one;
 //  - half a warp holds a block, eight elements a lane in two groups of four,
@@ -1022,9 +1045,12 @@ k_adamw8(const __grid_constant__ AdamwTable<N> tab, const __grid_constant__ Adam
         else if (d.grad_type == GS_TYPE_F32) adamw8_typed<GS_TYPE_F32, false>(d, now, st[at], a, h, s, tkey, lane);
         else if (d.grad_type == GS_TYPE_BF16) adamw8_typed<GS_TYPE_BF16, false>(d, now, st[at], a, h, s, tkey, lane);
         else adamw8_typed<GS_TYPE_F16, false>(d, now, st[at], a, h, s, tkey, lane);
-      } else {
-        const int full = d.vec != kScalar ? (int)min((d.count - now.tile) / kChunk8, (long long)kWarps8) : 0;
-        adamw_blocks<8>(d, now.tile, full, kWarps8, kChunk8, a, h, s, tkey);
+      }
+      if (d.vec == kScalar) {
+        adamw_blocks<8, kWarps8>(d, now.tile, 0, a, h, s, tkey);
+      } else if (d.count - now.tile < kAdamwTile) {
+        // what is left of the tensor behind its chunks, at most a block a warp
+        adamw_blocks<8, kWarps8>(d, now.tile, (int)(d.count - now.tile) / kChunk8, a, h, s, tkey);
       }
       __syncwarp();  // the stage has been read before it is copied into again
       now = next;
@@ -1108,10 +1134,9 @@ static int describe(const GsAdamwTensor& t, int index, int bits, AdamwDesc out[2
 template <int BITS, int N>
 static void launch_adamw_class(const GsAdamwTensor* t, int n, int index0, const AdamwParams& a, cudaStream_t st) {
   static thread_local AdamwTable<N> tab;
-  // one block a warp while that fills the SMs at most GS_ADAMW_SMALL times
   long long blocks = 0;
   for (int i = 0; i < n; ++i) blocks += (t[i].count + kAdamwBlock - 1) / kAdamwBlock;
-  const bool small = blocks <= (long long)device_sms() * GS_ADAMW_SMALL;
+  const bool small = blocks <= (long long)device_sms() * (BITS == 8 ? GS_ADAMW8_SMALL : GS_ADAMW_SMALL);
   const int tile = small ? kSmallWarps * kAdamwBlock : kAdamwTile;
   int tiles = 0, entries = 0;
   bool loose = false;
@@ -1322,7 +1347,6 @@ static int fill_grad_table(const GsGradTensor* t, int n, GradTable<N>& tab) {
   return tiles;
 }
 
-
 size_t grad_norm_workspace_bytes(int n) {
   const size_t launches = n > 0 ? ((size_t)n + kNormMost - 1) / kNormMost : 1;
   return launches * kNormGrid * sizeof(double);
@@ -1361,8 +1385,9 @@ void launch_grad_norm(const GsGradTensor* tensors, int n, float max_norm, const 
 }
 
 // ---------------------------------------------------------------------------
-// 8-bit moments to and from values, one warp a block. Encoding rounds to
-// nearest (halves up): values that came from codes are kept exactly.
+// 8-bit moments to and from values. Encoding rounds to nearest (halves up):
+// the values of a block's codes are kept exactly. Decoding 236M elements to
+// bf16: 245 us (6 B an element: 5.8 TB/s).
 __device__ __forceinline__ void store_value(float* p, float x) { *p = x; }
 __device__ __forceinline__ void store_value(__nv_bfloat16* p, float x) { *p = __float2bfloat16_rn(x); }
 
