@@ -5,7 +5,9 @@
  * Conventions
  *  - Every pointer argument is a DEVICE pointer unless its comment says "host".
  *  - All arrays are fp32 / int32 / uint8, C-contiguous, row-major, with the
- *    shapes of the reference arrays they replace (N = static capacity).
+ *    shapes of the reference arrays they replace (N = static capacity);
+ *    gs_adamw_step, gs_grad_norm and gs_moments8_decode also take 16-bit
+ *    floats.
  *  - No entry point allocates device memory, synchronises the stream or keeps
  *    global mutable state: scratch comes from a caller-owned `workspace` of at
  *    least gs_workspace_bytes(...) bytes, and all work is ordered on `stream`.

@@ -266,9 +266,10 @@ def _dev_tensor(x, like: torch.Tensor) -> torch.Tensor:
 def _step(state: DensityState, target_image, w2c, camera_static, optimizer: AdamConfig,
           sh_degree: int, group, capacity: Optional[int], lambda_ssim: float = 0.2,
           fused: bool = True):
-    if optimizer.moment_bits != state.moment_bits:
-        raise ValueError(f"the state's moments have {state.moment_bits} bits, the optimizer's {optimizer.moment_bits}")
-    if group is not None and fused and not optimizer.is_adam:
+    bits = getattr(optimizer, "moment_bits", 32)
+    if bits != state.moment_bits:
+        raise ValueError(f"the state's moments have {state.moment_bits} bits, the optimizer's {bits}")
+    if group is not None and fused and not getattr(optimizer, "is_adam", True):
         raise ValueError("the fused data-parallel update is plain Adam with 32-bit moments: use fused=False with "
                          "weight decay, max_grad_norm or 8-bit moments")
     W, H, fx, fy, cx, cy = camera_static
@@ -354,7 +355,7 @@ def _update(state: DensityState, optimizer: AdamConfig, mask: torch.Tensor, st: 
     """The update from the gradients in state.grads (trainer.py:73-77 /
     139-141): plain Adam, or AdamW where the optimizer asks for more."""
     state.count += 1
-    if not optimizer.is_adam:
+    if not getattr(optimizer, "is_adam", True):
         state.adamw(optimizer).step()
         return
     P = _lib.ptr
