@@ -143,7 +143,7 @@ struct AdamwParams {
 };
 
 __device__ __forceinline__ unsigned mix32(unsigned x) {
-  // lowbias32, C. Wellons, "Prospecting for Hash Functions" (2018)
+  // an integer hash from C. Wellons, "Prospecting for Hash Functions" (2018)
   x ^= x >> 16;
   x *= 0x7feb352du;
   x ^= x >> 15;

@@ -694,3 +694,79 @@ def test_no_tensors_is_a_step():
     _lib.call("gs_adamw_step", None, 0, ctypes.byref(cfg), None, _lib.ptr(state), _lib.stream(state.device))
     _lib.call("gs_grad_norm", None, 0, 1.0, None, _lib.ptr(out), _lib.ptr(ws), ws.numel(), _lib.stream(state.device))
     assert state.tolist() == [1, 0, 0, 0] and out[:2].tolist() == [0.0, 1.0]
+
+
+def test_far_elements_and_rows():
+    """32-bit moments, row mask and norm past 2^31 elements."""
+    from gs_b200.training.optimizer import AdamW, GradNorm, ParamTensor
+    w = 32_768
+    rows = (1 << 31) // w + 3
+    p = torch.zeros((rows, w), device="cuda")
+    g = torch.zeros((rows, w), dtype=torch.bfloat16, device="cuda")
+    mask = torch.ones(rows, dtype=torch.bool, device="cuda")
+    mask[-2] = False
+    rng = np.random.default_rng(0)
+    last = torch.tensor(rng.standard_normal((3, w)).astype(np.float32)).cuda()
+    g[-3:] = last
+    g[0, 0] = 2.0
+    arrays = [g[-3:].float().cpu().numpy(), np.float32([2.0])]
+    np.testing.assert_allclose(GradNorm([g])().cpu().numpy()[0], R.grad_norm(arrays)[0], rtol=2.0 ** -23)
+    opt = AdamW([ParamTensor(p, g, lr=1e-2, active=mask)])
+    opt.step()
+    (mu, nu), = opt.moment_values()
+    z = np.zeros(3 * w, np.float32)
+    m, v = R.moments(z, z, arrays[0].reshape(-1), 1.0, 0.9, 0.999)
+    want, err = R.param(z, m, v, 0, 1e-2, 0.0, 0.9, 0.999, 1e-8, np.repeat([True, False, True], w))
+    assert (np.abs(p[-3:].cpu().numpy().reshape(-1) - want) <= err).all()
+    np.testing.assert_array_equal(mu[-3:].cpu().numpy().reshape(-1), m)
+    np.testing.assert_array_equal(nu[-3:].cpu().numpy().reshape(-1), v)
+    assert float(p[1:1000].abs().max()) == 0.0 and abs(float(p[0, 0]) + 1e-2) < 1e-6
+    del p, g, opt, mu, nu
+    torch.cuda.empty_cache()
+
+
+def test_plans_on_threads_and_streams():
+    """Plans of their own on two host threads and two streams, eager and as graphs, end as they do one after the other."""
+    import threading
+
+    def run(seed, steps):
+        s = Setup([150_001, 700, 33], 8 if seed % 2 else 32, seed=seed, max_grad_norm=0.5)
+        for _ in range(steps):
+            s.opt.step()
+        return s
+
+    want = [run(seed, 40) for seed in (1, 2)]
+    torch.cuda.synchronize()
+    got, errors = {}, []
+
+    def work(seed):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                got[seed] = run(seed, 40)
+                torch.cuda.current_stream().synchronize()
+        except Exception as e:  # noqa: BLE001 -- shown by the assertion below
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=(seed,)) for seed in (1, 2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors, errors
+    both = [run(seed, 1) for seed in (1, 2)]
+    torch.cuda.synchronize()
+    streams, graphs = [torch.cuda.Stream() for _ in both], []
+    for s in both:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            s.opt.step()
+    for _ in range(39):
+        for stream, graph in zip(streams, graphs):
+            with torch.cuda.stream(stream):
+                graph.replay()
+    torch.cuda.synchronize()
+    for a, b, c in zip(want, (got[1], got[2]), both):
+        for x, y, z in zip(a.read(), b.read(), c.read()):
+            for i in range(4):
+                np.testing.assert_array_equal(x[i], y[i])
+                np.testing.assert_array_equal(x[i], z[i])
