@@ -444,6 +444,22 @@ GS_API int gs_density_step_stats(const float* grad_means, const float* means, co
                                  float* grad2d, gs_stream_t stream);
 
 /*
+ * The same two with a gate (device float, nullable): while *gate is not
+ * finite, grad_accum, denom and max_radii stay as they are. With the clip
+ * factor of gs_grad_norm, a step that gs_adamw_step skips leaves no statistics
+ * behind either. grad2d is written all the same.
+ */
+GS_API int gs_density_step_stats_gated(const float* grad_means, const float* means, const float* w2c, int n,
+                                       float fx, float fy, int width, int height, const float* radii,
+                                       const uint8_t* valid, const uint8_t* active, const float* gate,
+                                       float* grad_accum, int32_t* denom, float* max_radii, float* grad2d,
+                                       gs_stream_t stream);
+GS_API int gs_accumulate_density_stats_gated(const float* grad2d, const float* radii, const uint8_t* valid,
+                                             const uint8_t* radii_valid, const uint8_t* active, int n,
+                                             const float* gate, float* grad_accum, int32_t* denom,
+                                             float* max_radii, gs_stream_t stream);
+
+/*
  * The train step's returned loss and metrics (trainer.py:18-26 and the
  * metrics dict of train_step_internal) packed by one small kernel: from
  * tail = [l1, d_ssim, ...] writes out[0] = (1 - lambda) l1 + lambda d_ssim,

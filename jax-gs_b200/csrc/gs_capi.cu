@@ -768,10 +768,18 @@ int gs_density_step_stats(const float* grad_means, const float* means, const flo
                           float fy, int width, int height, const float* radii, const uint8_t* valid,
                           const uint8_t* active, float* grad_accum, int32_t* denom, float* max_radii,
                           float* grad2d, gs_stream_t stream) {
+  return gs_density_step_stats_gated(grad_means, means, w2c, n, fx, fy, width, height, radii, valid, active, nullptr,
+                                     grad_accum, denom, max_radii, grad2d, stream);
+}
+
+int gs_density_step_stats_gated(const float* grad_means, const float* means, const float* w2c, int n, float fx,
+                                float fy, int width, int height, const float* radii, const uint8_t* valid,
+                                const uint8_t* active, const float* gate, float* grad_accum, int32_t* denom,
+                                float* max_radii, float* grad2d, gs_stream_t stream) {
   if (n < 0 || width <= 0 || height <= 0) return GS_ERR_INVALID_ARGUMENT;
   if (n > 0 && (!grad_means || !means || !w2c || !radii || !valid || !grad_accum || !denom || !max_radii))
     return GS_ERR_INVALID_ARGUMENT;
-  launch_step_stats(grad_means, means, w2c, n, fx, fy, width, height, radii, valid, active, grad_accum, denom,
+  launch_step_stats(grad_means, means, w2c, n, fx, fy, width, height, radii, valid, active, gate, grad_accum, denom,
                     max_radii, grad2d, (cudaStream_t)stream);
   return last_error();
 }
@@ -780,10 +788,17 @@ int gs_accumulate_density_stats(const float* grad2d, const float* radii, const u
                                 const uint8_t* radii_valid, const uint8_t* active, int n,
                                 float* grad_accum, int32_t* denom, float* max_radii,
                                 gs_stream_t stream) {
+  return gs_accumulate_density_stats_gated(grad2d, radii, valid, radii_valid, active, n, nullptr, grad_accum, denom,
+                                           max_radii, stream);
+}
+
+int gs_accumulate_density_stats_gated(const float* grad2d, const float* radii, const uint8_t* valid,
+                                      const uint8_t* radii_valid, const uint8_t* active, int n, const float* gate,
+                                      float* grad_accum, int32_t* denom, float* max_radii, gs_stream_t stream) {
   if (n < 0) return GS_ERR_INVALID_ARGUMENT;
   if (n > 0 && (!grad2d || !radii || !valid || !grad_accum || !denom || !max_radii))
     return GS_ERR_INVALID_ARGUMENT;
-  launch_density_stats(grad2d, radii, valid, radii_valid ? radii_valid : valid, active, n, grad_accum,
+  launch_density_stats(grad2d, radii, valid, radii_valid ? radii_valid : valid, active, n, gate, grad_accum,
                        denom, max_radii, stream);
   return last_error();
 }

@@ -251,9 +251,10 @@ void launch_step_metrics(const float* tail, const GsExtras* ex, float lambda, co
                          cudaStream_t st);
 void launch_step_stats(const float* grad_means, const float* means, const float* w2c, int n, float fx, float fy,
                        int width, int height, const float* radii, const uint8_t* valid, const uint8_t* active,
-                       float* grad_accum, int32_t* denom, float* max_radii, float* grad2d, cudaStream_t st);
+                       const float* gate, float* grad_accum, int32_t* denom, float* max_radii, float* grad2d,
+                       cudaStream_t st);
 void launch_density_stats(const float* grad2d, const float* radii, const uint8_t* valid,
-                          const uint8_t* radii_valid, const uint8_t* active, int n,
+                          const uint8_t* radii_valid, const uint8_t* active, int n, const float* gate,
                           float* grad_accum, int32_t* denom, float* max_radii, cudaStream_t st);
 
 // gs_adamw.cu: AdamW over many tensors, the gradient norm, 8-bit moments

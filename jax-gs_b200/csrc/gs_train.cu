@@ -329,15 +329,19 @@ void launch_grad2d(const float* grad_means, const float* means, const float* w2c
   launch_kernel_plain(k_grad2d, nb, 256, 0, st, grad_means, means, w2c, n, focal, pix3, out);
 }
 
+// Whether the step counts: no gate, or one that is finite (the clip's factor,
+// NaN where gs_adamw_step skips the step).
+__device__ __forceinline__ bool gate_open(const float* gate) { return !gate || fabsf(__ldg(gate)) <= 3.402823466e38f; }
+
 // grad_accum / denom / max_radii updates (trainer.py:100-113, :152-159).
 __global__ void __launch_bounds__(256)
 k_density_stats(const float* __restrict__ grad2d, const float* __restrict__ radii,
                 const uint8_t* __restrict__ valid, const uint8_t* __restrict__ radii_valid,
-                const uint8_t* __restrict__ active, int n, float* __restrict__ grad_accum,
-                int32_t* __restrict__ denom, float* __restrict__ max_radii) {
+                const uint8_t* __restrict__ active, int n, const float* __restrict__ gate,
+                float* __restrict__ grad_accum, int32_t* __restrict__ denom, float* __restrict__ max_radii) {
   GS_PDL_ENTRY_PLAIN();
   const int i = blockIdx.x * 256 + threadIdx.x;
-  if (i >= n) return;
+  if (i >= n || !gate_open(gate)) return;
   grad_accum[i] = grad_accum[i] + grad2d[i];
   const bool a = active ? (active[i] != 0) : true;
   if (valid[i] != 0 && a) denom[i] = denom[i] + 1;
@@ -350,8 +354,8 @@ k_density_stats(const float* __restrict__ grad2d, const float* __restrict__ radi
 __global__ void __launch_bounds__(256)
 k_step_stats(const float* __restrict__ gmeans, const float* __restrict__ means, const float* __restrict__ w2c,
              int n, float focal, float pix3, const float* __restrict__ radii, const uint8_t* __restrict__ valid,
-             const uint8_t* __restrict__ active, float* __restrict__ grad_accum, int32_t* __restrict__ denom,
-             float* __restrict__ max_radii, float* __restrict__ grad2d_out) {
+             const uint8_t* __restrict__ active, const float* __restrict__ gate, float* __restrict__ grad_accum,
+             int32_t* __restrict__ denom, float* __restrict__ max_radii, float* __restrict__ grad2d_out) {
   GS_PDL_ENTRY_PLAIN();
   const int i = blockIdx.x * 256 + threadIdx.x;
   if (i >= n) return;
@@ -364,6 +368,7 @@ k_step_stats(const float* __restrict__ gmeans, const float* __restrict__ means, 
   const float nrm = sqrtf(g0 * g0 + g1 * g1 + g2 * g2);
   const float g2d = (nrm * (z / focal)) * pix3;
   if (grad2d_out) grad2d_out[i] = g2d;
+  if (!gate_open(gate)) return;
   grad_accum[i] = grad_accum[i] + g2d;
   const bool v = valid[i] != 0;
   const bool a = active ? (active[i] != 0) : true;
@@ -373,24 +378,25 @@ k_step_stats(const float* __restrict__ gmeans, const float* __restrict__ means, 
 
 void launch_step_stats(const float* grad_means, const float* means, const float* w2c, int n, float fx, float fy,
                        int width, int height, const float* radii, const uint8_t* valid, const uint8_t* active,
-                       float* grad_accum, int32_t* denom, float* max_radii, float* grad2d, cudaStream_t st) {
+                       const float* gate, float* grad_accum, int32_t* denom, float* max_radii, float* grad2d,
+                       cudaStream_t st) {
   const int nb = (n + 255) / 256;
   if (nb == 0) return;
   const float focal = (float)(((double)fx + (double)fy) / 2.0);
   const float pix3 = (float)((double)width * (double)height * 3.0);
   GS_TIMED("step_stats", st);
-  launch_kernel_plain(k_step_stats, nb, 256, 0, st, grad_means, means, w2c, n, focal, pix3, radii, valid, active, grad_accum, denom,
-                                    max_radii, grad2d);
+  launch_kernel_plain(k_step_stats, nb, 256, 0, st, grad_means, means, w2c, n, focal, pix3, radii, valid, active, gate, grad_accum,
+                                    denom, max_radii, grad2d);
 }
 
 void launch_density_stats(const float* grad2d, const float* radii, const uint8_t* valid,
-                          const uint8_t* radii_valid, const uint8_t* active, int n,
+                          const uint8_t* radii_valid, const uint8_t* active, int n, const float* gate,
                           float* grad_accum, int32_t* denom, float* max_radii, cudaStream_t st) {
   int nb = (n + 255) / 256;
   if (nb == 0) return;
   GS_TIMED("density_stats", st);
-  launch_kernel_plain(k_density_stats, nb, 256, 0, st, grad2d, radii, valid, radii_valid, active, n, grad_accum, denom,
-                                       max_radii);
+  launch_kernel_plain(k_density_stats, nb, 256, 0, st, grad2d, radii, valid, radii_valid, active, n, gate, grad_accum,
+                                       denom, max_radii);
 }
 
 }  // namespace gs

@@ -131,6 +131,8 @@ SIGNATURES = {
     "gs_grad2d_magnitude": (_I, [_P, _P, _P, _I, _F, _F, _I, _I, _P, _P]),
     "gs_accumulate_density_stats": (_I, [_P, _P, _P, _P, _P, _I, _P, _P, _P, _P]),
     "gs_density_step_stats": (_I, [_P, _P, _P, _I, _F, _F, _I, _I, _P, _P, _P, _P, _P, _P, _P, _P]),
+    "gs_density_step_stats_gated": (_I, [_P, _P, _P, _I, _F, _F, _I, _I, _P, _P, _P, _P, _P, _P, _P, _P, _P]),
+    "gs_accumulate_density_stats_gated": (_I, [_P, _P, _P, _P, _P, _I, _P, _P, _P, _P, _P]),
     "gs_adamw_step": (_I, [ctypes.POINTER(GsAdamwTensor), _I, ctypes.POINTER(GsAdamwConfig), _P, _P, _P]),
     "gs_grad_norm": (_I, [ctypes.POINTER(GsGradTensor), _I, _F, _P, _P, _P, _S, _P]),
     "gs_grad_norm_workspace_bytes": (_S, [_I]),

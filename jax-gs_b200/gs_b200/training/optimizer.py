@@ -371,8 +371,19 @@ class AdamW(_Plan):
 
     def step(self) -> None:
         """One step on the gradients as they are."""
+        self.clip()
+        self.update()
+
+    def clip(self) -> Optional[torch.Tensor]:
+        """The first half of step(): the gradients' norm, with max_grad_norm.
+        Returns grad_scale, the device value while which is not finite
+        update() changes nothing (None: nothing is skipped)."""
         if self.norm is not None:
             self.norm()
+        return self.grad_scale
+
+    def update(self) -> None:
+        """The second half of step(): parameters, moments and copies."""
         self._call("gs_adamw_step", *self._args)
         # the library writes through raw pointers: tell autograd, as an in-place operation does
         torch.autograd.graph.increment_version(self._bumped)

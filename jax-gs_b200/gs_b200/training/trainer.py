@@ -48,8 +48,8 @@ class AdamConfig:
     from its default the step updates through gs_adamw_step
     (gs_b200.training.optimizer): decoupled weight decay per group [means,
     scales, quaternions, opacities, sh], a clip by the global norm of the
-    gradient (a step whose gradient is not finite is then skipped, counted in
-    DensityState.skipped), Adam moments in 8 bits (a quarter of the memory),
+    gradient (a step whose gradient is not finite is then skipped, densification
+    statistics included, and counted in DensityState.skipped), Adam moments in 8 bits (a quarter of the memory),
     and the seed of their stochastic rounding."""
     means_lr_init: float = 0.00016 * 3.0
     means_lr_end: float = 0.0000016 * 3.0
@@ -333,8 +333,9 @@ def _step(state: DensityState, target_image, w2c, camera_static, optimizer: Adam
     if group is None:
         # single device: grad_2d_mag (pre-update means) and the densification
         # statistics (trainer.py:143-159) in one kernel, then Adam
-        _lib.call("gs_density_step_stats", P(gf.means), P(p.means), P(w2c_d), n, fx, fy, W, H, P(radii), P(valid),
-                  P(mask), P(state.grad_accum), P(state.denom), P(state.max_radii), None, st)
+        gate = _clip(state, optimizer)
+        _lib.call("gs_density_step_stats_gated", P(gf.means), P(p.means), P(w2c_d), n, fx, fy, W, H, P(radii),
+                  P(valid), P(mask), P(gate), P(state.grad_accum), P(state.denom), P(state.max_radii), None, st)
         _update(state, optimizer, mask, st)
         return b
     pmean_gradients(state.grads, tail, b["extras"], group)
@@ -343,20 +344,30 @@ def _step(state: DensityState, target_image, w2c, camera_static, optimizer: Adam
     radii, radii_valid = pmean_grad2d_pmax_radii(b["g2d"], radii, valid, group)
     # Adam + masking + apply (trainer.py:73-77 / 139-141); the schedule is
     # evaluated on the device from state.adam_state so a graph can replay it
+    gate = _clip(state, optimizer)
     _update(state, optimizer, mask, st)
     # densification statistics (trainer.py:100-113 / 152-159)
     # denom counts this rank's own visibility; max_radii uses the max over ranks
-    _lib.call("gs_accumulate_density_stats", P(b["g2d"]), P(radii), P(valid), P(radii_valid), P(mask),
-              n, P(state.grad_accum), P(state.denom), P(state.max_radii), st)
+    _lib.call("gs_accumulate_density_stats_gated", P(b["g2d"]), P(radii), P(valid), P(radii_valid), P(mask),
+              n, P(gate), P(state.grad_accum), P(state.denom), P(state.max_radii), st)
     return b
+
+
+def _clip(state: DensityState, optimizer: AdamConfig) -> Optional[torch.Tensor]:
+    """The norm of the gradients in state.grads, if the optimizer clips by it.
+    Returns the device value that is not finite when the update will skip the
+    step, whose statistics are then not to be taken either (None: it never
+    does)."""
+    return None if getattr(optimizer, "is_adam", True) else state.adamw(optimizer).clip()
 
 
 def _update(state: DensityState, optimizer: AdamConfig, mask: torch.Tensor, st: int) -> None:
     """The update from the gradients in state.grads (trainer.py:73-77 /
-    139-141): plain Adam, or AdamW where the optimizer asks for more."""
+    139-141): plain Adam, or AdamW where the optimizer asks for more (after
+    _clip)."""
     state.count += 1
     if not getattr(optimizer, "is_adam", True):
-        state.adamw(optimizer).step()
+        state.adamw(optimizer).update()
         return
     P = _lib.ptr
     sched = optimizer.schedule()
