@@ -145,12 +145,23 @@ class DensityState:
         self.grad_accum = torch.zeros(self.n, **f)
         self.denom = torch.zeros(self.n, dtype=torch.int32, device=self.device)
         self.max_radii = torch.zeros(self.n, **f)
-        self.count = 0  # optax step count (host mirror)
+        self._count, self._may_skip = 0, False  # steps given to the device; whether it may have skipped some
         # device [optax count, ticket] read and advanced by gs_adam_step_scheduled
         # and gs_adamw_step; then the steps that one skipped, and 0
         self.adam_state = torch.zeros(4, dtype=torch.int32, device=self.device)
         self._buffers: Dict = {}
         self._adamw = None  # (hyperparameters, plan) of the last AdamW update
+
+    @property
+    def count(self) -> int:
+        """The optax step count: the host's mirror of adam_state[0]. Once a
+        step had a clip only the device knows which ones were skipped, so it
+        is read from there (synchronises)."""
+        return int(self.adam_state[0]) if self._may_skip else self._count
+
+    @count.setter
+    def count(self, steps: int) -> None:
+        self._count = int(steps)
 
     @property
     def skipped(self) -> torch.Tensor:
@@ -321,13 +332,13 @@ def _step(state: DensityState, target_image, w2c, camera_static, optimizer: Adam
         # gradient average + Adam + statistics over NVLink peer memory (the
         # update reads every rank's render counters from its extras)
         dp.barrier(touched)  # every rank's gradients (and touched flags) are final
-        state.count += 1
         sched = optimizer.schedule()
         # a rendezvous that gave up (dp.status != 0) makes the update touch no
         # peer memory and change nothing; the step's metrics report it
         _lib.call("gs_dp_update", ctypes.byref(dp.peers), P(state.mu), P(state.nu), n, k, P(mask),
                   ctypes.byref(sched), P(state.adam_state), fx, fy, W, H, TAIL, P(dp.tail_out),
                   P(dp.status), st)
+        state._count += 1
         dp.barrier()  # every rank's peer writes are done
         return b
     if group is None:
@@ -365,14 +376,15 @@ def _update(state: DensityState, optimizer: AdamConfig, mask: torch.Tensor, st: 
     """The update from the gradients in state.grads (trainer.py:73-77 /
     139-141): plain Adam, or AdamW where the optimizer asks for more (after
     _clip)."""
-    state.count += 1
     if not getattr(optimizer, "is_adam", True):
         state.adamw(optimizer).update()
-        return
-    P = _lib.ptr
-    sched = optimizer.schedule()
-    _lib.call("gs_adam_step_scheduled", P(state.params), P(state.grads), P(state.mu), P(state.nu), state.n,
-              state.sh_k, P(mask), ctypes.byref(sched), P(state.adam_state), st)
+        state._may_skip |= optimizer.max_grad_norm is not None
+    else:
+        P = _lib.ptr
+        sched = optimizer.schedule()
+        _lib.call("gs_adam_step_scheduled", P(state.params), P(state.grads), P(state.mu), P(state.nu), state.n,
+                  state.sh_k, P(mask), ctypes.byref(sched), P(state.adam_state), st)
+    state._count += 1
 
 
 def pmean_gradients(grads: torch.Tensor, tail: torch.Tensor, extras: torch.Tensor, group) -> None:
@@ -626,7 +638,7 @@ class CapturedStep:
             _step(state, self.target, self.w2c, camera_static, optimizer, sh_degree, group, capacity,
                   fused=fused)
             self.loss, self.metrics = _loss_metrics(state, b, group, fused)
-        self.state.count -= 1  # the capture did not run the step
+        self.state._count -= 1  # the capture did not run the step
         self._plan = state._adamw[1] if state._adamw else None  # the graph holds its buffers' addresses
         self._stager = InputStager(state.device)  # host inputs upload during the previous step
 
@@ -634,6 +646,6 @@ class CapturedStep:
         self._stager.upload([torch.as_tensor(target_image, dtype=torch.float32),
                              torch.as_tensor(w2c, dtype=torch.float32)], [self.target, self.w2c])
         self.graph.replay()
-        self.state.count += 1
+        self.state._count += 1
         return self.state, self.loss, self.metrics
 
