@@ -396,8 +396,9 @@ class AdamW(_Plan):
         return [(m.view(t.param.shape), v.view(t.param.shape)) for m, v, t in zip(mu, nu, self.tensors)]
 
     def state_dict(self) -> Dict:
-        """Copies of the step count, the steps skipped and the moments."""
+        """Copies of the step count, the steps skipped and the moments, with the tensors' sizes."""
         return {"state": self._state.clone(), "moment_bits": self.moment_bits,
+                "sizes": [t.param.numel() for t in self.tensors],
                 "moments": [t.clone() for t in self._moment_buffers()]}
 
     def load_state_dict(self, state: Dict) -> None:
@@ -405,7 +406,11 @@ class AdamW(_Plan):
         buffers = self._moment_buffers()
         if state["moment_bits"] != self.moment_bits:
             raise ValueError("moment_bits differ")
-        if [t.numel() for t in state["moments"]] != [t.numel() for t in buffers]:
+        # 8-bit moments lie in flat buffers, whose lengths do not tell the tensors' order (a state saved without its
+        # sizes is taken by the lengths)
+        sizes = [t.param.numel() for t in self.tensors]
+        if (state.get("sizes", sizes) != sizes
+                or [t.numel() for t in state["moments"]] != [t.numel() for t in buffers]):
             raise ValueError("sizes of the moments differ")
         self._state.copy_(state["state"])
         for t, s in zip(buffers, state["moments"]):
