@@ -36,7 +36,8 @@ class ParamTensor:
 
     param is float32; grad has its number of elements in float32, bfloat16 or
     float16. The learning rate of the step that follows c others is
-    lr * lr_decay_rate ** (c / lr_transition_steps) (optax.exponential_decay).
+    lr * lr_decay_rate ** (c / lr_transition_steps) (optax.exponential_decay;
+    with a rate of 0, lr for the first step and 0 from then on).
     active (bool or uint8, one flag per row of param's first dimension): rows
     whose flag is 0 keep their parameter. copy (bfloat16 or float16) receives
     the new parameter, rounded.
@@ -368,6 +369,10 @@ class AdamW(_Plan):
         for d, t in zip(self._table, self.tensors):
             d.lr_init, d.weight_decay = float(t.lr), float(t.weight_decay)
             d.decay_rate, d.transition_steps = float(t.lr_decay_rate), float(t.lr_transition_steps)
+            if d.decay_rate == 0.0 and d.transition_steps > 0.0:
+                # 0 ^ (c / steps) is 1 at c = 0 and 0 behind it, as is 2^-126 ^ (1024 c) in float32: the library
+                # takes the logarithm of the rate
+                d.decay_rate, d.transition_steps = 2.0 ** -126, 2.0 ** -10
 
     def step(self) -> None:
         """One step on the gradients as they are."""
