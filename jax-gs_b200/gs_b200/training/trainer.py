@@ -49,8 +49,11 @@ class AdamConfig:
     (gs_b200.training.optimizer): decoupled weight decay per group [means,
     scales, quaternions, opacities, sh], a clip by the global norm of the
     gradient (a step whose gradient is not finite is then skipped, densification
-    statistics included, and counted in DensityState.skipped), Adam moments in 8 bits (a quarter of the memory),
-    and the seed of their stochastic rounding."""
+    statistics included, and counted in DensityState.skipped), Adam moments in 8
+    bits (a quarter of the memory), and the seed of their stochastic rounding.
+    An eps from 0 to below float32's smallest normal number then counts as that
+    number: rows with a second moment move as with eps = 0, rows without one
+    stay (plain Adam's 0 / 0 makes them NaN)."""
     means_lr_init: float = 0.00016 * 3.0
     means_lr_end: float = 0.0000016 * 3.0
     transition_steps: int = 30000
@@ -176,7 +179,11 @@ class DensityState:
     def adamw(self, optimizer: AdamConfig) -> AdamW:
         """The AdamW plan over the five groups (kept until the hyperparameters
         change; changed rates are taken over)."""
-        hyper = (optimizer.b1, optimizer.b2, optimizer.eps, optimizer.max_grad_norm, optimizer.moment_seed)
+        # gs_adamw_step divides by numbers that are at least eps and wants it normal; any root of a second moment that
+        # is not 0 (2^-74.5 and above) swallows the smallest one
+        tiny = torch.finfo(torch.float32).tiny
+        eps = tiny if 0.0 <= optimizer.eps < tiny else optimizer.eps
+        hyper = (optimizer.b1, optimizer.b2, eps, optimizer.max_grad_norm, optimizer.moment_seed)
         lrs, wd = optimizer.lrs(0), [float(w) for w in optimizer.weight_decay]
         if len(wd) != 5:
             raise ValueError("weight_decay: one value for each of the five groups")
@@ -190,7 +197,7 @@ class DensityState:
             moments = self.moments8
             if moments is None:
                 moments = [(rows(self.mu, i), rows(self.nu, i)) for i in range(5)]
-            plan = AdamW(tensors, b1=optimizer.b1, b2=optimizer.b2, eps=optimizer.eps, moments=moments,
+            plan = AdamW(tensors, b1=optimizer.b1, b2=optimizer.b2, eps=eps, moments=moments,
                          max_grad_norm=optimizer.max_grad_norm, seed=optimizer.moment_seed, state=self.adam_state)
             self._adamw = [hyper, plan, rates]
         _, plan, known = self._adamw

@@ -3,7 +3,8 @@ import numpy as np
 import pytest
 import torch
 
-from tests.test_gpu_adamw_train import _state
+from tests import adamw_ref as A
+from tests.test_gpu_adamw_train import _moments, _state
 
 pytestmark = pytest.mark.gpu
 
@@ -35,3 +36,30 @@ def test_adamw_takes_a_decay_rate_of_zero():
         np.testing.assert_allclose(after.cpu().numpy(), 0.5, rtol=0, atol=0.5 * 57 * 2.0 ** -24)
         opt.step()
         assert torch.equal(p, after) and int(opt.count) == 2
+
+
+@pytest.mark.parametrize("eps", [0.0, 1e-45, 1e-38, 1e-60])
+@pytest.mark.parametrize("bits", [32, 8])
+def test_an_eps_below_the_smallest_normal_number(eps, bits):
+    """It counts as that number: rows with a second moment move as with eps = 0 (|root| is at least 2^-74.5, far
+    above), rows without one stay."""
+    from gs_b200.training.trainer import train_step
+    st, opt, cam, views = _state(max_grad_norm=1e6, moment_bits=bits)
+    opt.eps = eps
+    for c, view in enumerate(views[:2]):
+        p0 = st.params.cpu().numpy()
+        m0, v0 = _moments(st)
+        train_step(st, *view, cam, opt, sh_degree=3)
+        m, v = A.moments(m0, v0, st.grads[:st.size].cpu().numpy(), st._adamw[1].norm.scale.cpu().numpy(), opt.b1, opt.b2)
+        p1 = st.params.cpu().numpy()
+        assert np.isfinite(p1).all()
+        lrs = opt.lrs(c)
+        rows = st.active_mask.cpu().numpy()
+        for i, (a, b) in enumerate(st.segments):
+            s = slice(a, b)
+            act = np.repeat(rows, (b - a) // st.n)
+            seen = v[s] > 0
+            want, err = A.param(p0[s], m[s], v[s], c, lrs[i], 0.0, opt.b1, opt.b2, 0.0, act)
+            assert (np.abs(p1[s] - want) <= err)[seen].all(), i
+            still = (v[s] == 0) & (m[s] == 0)
+            assert still.any() and (p1[s][still] == p0[s][still]).all()
