@@ -682,6 +682,20 @@ GS_API int gs_densify_and_prune(float* params, float* mu, float* nu, int n, int 
 GS_API size_t gs_density_workspace_bytes(int n);
 
 /*
+ * The same with the moments in 8 bits (mu, nu codes and their exponent bytes
+ * as in GsAdamwTensor, each of the five groups from the next multiple of 128
+ * elements): blocks that receive rows are rounded to nearest again, the others
+ * stay as they are. Workspace: gs_density8_workspace_bytes(N, K) bytes,
+ * 256-byte aligned, which hold a copy of one moment's codes.
+ */
+GS_API int gs_densify_and_prune8(float* params, uint8_t* mu, uint8_t* nu, uint8_t* mu_exp, uint8_t* nu_exp, int n,
+                                 int sh_k, uint8_t* active_mask, float* grad_accum, int32_t* denom,
+                                 const float* max_radii, const float* noise, int densify_enabled,
+                                 float grad_threshold, float min_opacity, float extent, float max_screen_size,
+                                 void* workspace, size_t workspace_bytes, int32_t* info, gs_stream_t stream);
+GS_API size_t gs_density8_workspace_bytes(int n, int sh_k);
+
+/*
  * reset_opacities, density.py:76-96: the opacities of active Gaussians are
  * set to log(reset_val / (1 - reset_val)) (float32); moments unchanged.
  */

@@ -1528,4 +1528,98 @@ void launch_moments8_encode(const float* mu, const float* nu, long long count, u
   launch_kernel_plain(k_moments8_encode, grid, 256, 0, st, mu, nu, count, mu8, nu8, mu_exp, nu_exp);
 }
 
+// Rows of the five groups that move to other slots (density control), one
+// moment. A row's new block has another exponent, so a block that receives
+// rows is encoded again as a whole, to nearest; the others are not touched.
+// Values are read from a copy of the codes: a source may lie in a block that
+// is encoded again. 240k of 4M rows moved (236M elements):
+// both moments 1.35 ms, of which the copies are 0.2; the rest are the tests of
+// every element's row, and it runs once in a hundred steps.
+struct Moments8Groups {
+  int first[6];    // first block of each group
+  unsigned width[5];
+  unsigned count[5];  // elements
+};
+
+template <bool SIGNED>
+__global__ void __launch_bounds__(256)
+k_moments8_move(const uint8_t* __restrict__ from, const uint8_t* __restrict__ from_exp, uint8_t* __restrict__ codes,
+                uint8_t* __restrict__ exps, Moments8Groups g, const int* __restrict__ source) {
+  GS_PDL_ENTRY_PLAIN();
+  const int lane = threadIdx.x & 31;
+  for (int blk = blockIdx.x * 8 + (threadIdx.x >> 5); blk < g.first[5]; blk += gridDim.x * 8) {
+    int k = 0;
+#pragma unroll
+    for (int q = 1; q < 5; ++q)
+      if (blk >= g.first[q]) k = q;
+    const unsigned w = g.width[k], count = g.count[k], e0 = (unsigned)(blk - g.first[k]) * kAdamwBlock;
+    const size_t base = (size_t)g.first[k] * kAdamwBlock;
+    unsigned at[4];  // element of the group that each one takes its value from
+    bool moved = false;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const unsigned e = e0 + lane + 32 * q, row = e / w;
+      at[q] = e;
+      if (e >= count) continue;
+      const int src = source[row];
+      if (src < 0) continue;
+      at[q] = (unsigned)src * w + (e - row * w);
+      moved = true;
+    }
+    if (!__any_sync(0xffffffffu, moved)) continue;
+    float x[4];
+    unsigned top = 0u;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      x[q] = 0.f;
+      if (e0 + lane + 32 * q < count) {
+        const size_t i = base + at[q];
+        const int f = from_exp[i / kAdamwBlock];
+        x[q] = f == 255 ? NAN : decode8<SIGNED>(from[i], pow2_biased(f));
+      }
+      top = max(top, __float_as_uint(fabsf(x[q])));
+    }
+    const int f = block_field(__reduce_max_sync(0xffffffffu, top));
+    const float down = pow2_biased(max(254 - f, 0));
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const unsigned e = e0 + lane + 32 * q;
+      if (e < count) codes[base + e] = (uint8_t)(f == 255 ? 0u : encode8<SIGNED>(x[q], down, 1u << 19));
+    }
+    if (lane == 0) exps[blk] = (uint8_t)f;
+  }
+}
+
+static Moments8Groups moments8_groups(int n, int sh_k) {
+  const unsigned widths[5] = {3u, 3u, 4u, 1u, 3u * (unsigned)sh_k};
+  Moments8Groups g;
+  g.first[0] = 0;
+  for (int k = 0; k < 5; ++k) {
+    g.width[k] = widths[k];
+    g.count[k] = widths[k] * (unsigned)n;
+    g.first[k + 1] = g.first[k] + (int)((g.count[k] + kAdamwBlock - 1) / kAdamwBlock);
+  }
+  return g;
+}
+
+// A copy of one moment's codes and exponent bytes.
+size_t moments8_move_bytes(int n, int sh_k) { return (size_t)moments8_groups(n, sh_k).first[5] * (kAdamwBlock + 1); }
+
+void launch_moments8_move(uint8_t* mu, uint8_t* nu, uint8_t* mu_exp, uint8_t* nu_exp, int n, int sh_k,
+                          const int* source, void* ws, cudaStream_t st) {
+  const Moments8Groups g = moments8_groups(n, sh_k);
+  const size_t blocks = (size_t)g.first[5], codes = blocks * kAdamwBlock;
+  if (blocks == 0) return;
+  uint8_t *from = static_cast<uint8_t*>(ws), *from_exp = from + codes;
+  const int grid = (int)std::min<long long>(((long long)blocks + 7) / 8, (long long)device_sms() * 8);
+  GS_TIMED("moments8_move", st);
+  for (int moment = 0; moment < 2; ++moment) {
+    uint8_t *x = moment ? nu : mu, *f = moment ? nu_exp : mu_exp;
+    cudaMemcpyAsync(from, x, codes, cudaMemcpyDeviceToDevice, st);
+    cudaMemcpyAsync(from_exp, f, blocks, cudaMemcpyDeviceToDevice, st);
+    launch_kernel_plain(moment ? k_moments8_move<false> : k_moments8_move<true>, grid, 256, 0, st, from, from_exp, x,
+                        f, g, source);
+  }
+}
+
 }  // namespace gs

@@ -607,6 +607,31 @@ int gs_densify_and_prune(float* params, float* mu, float* nu, int n, int sh_k, u
   return last_error();
 }
 
+size_t gs_density8_workspace_bytes(int n, int sh_k) {
+  if (n < 0 || sh_k < 1 || sh_k > 16 || (long long)n * (11 + 3 * sh_k) > 0x7FFFFFFFll) return 0;
+  return density_workspace_bytes(n) + moments8_move_bytes(n, sh_k);
+}
+
+int gs_densify_and_prune8(float* params, uint8_t* mu, uint8_t* nu, uint8_t* mu_exp, uint8_t* nu_exp, int n, int sh_k,
+                          uint8_t* active_mask, float* grad_accum, int32_t* denom, const float* max_radii,
+                          const float* noise, int densify_enabled, float grad_threshold, float min_opacity,
+                          float extent, float max_screen_size, void* workspace, size_t workspace_bytes, int32_t* info,
+                          gs_stream_t stream) {
+  if (n < 0 || sh_k < 1 || sh_k > 16 || !info) return GS_ERR_INVALID_ARGUMENT;
+  if ((long long)n * (11 + 3 * sh_k) > 0x7FFFFFFFll) return GS_ERR_INVALID_ARGUMENT;
+  if (n > 0 && (!params || !mu || !nu || !mu_exp || !nu_exp || !active_mask || !grad_accum || !denom || !max_radii ||
+                !noise))
+    return GS_ERR_INVALID_ARGUMENT;
+  if (!workspace || workspace_bytes < gs_density8_workspace_bytes(n, sh_k) || (((uintptr_t)workspace) & 255))
+    return GS_ERR_WORKSPACE_TOO_SMALL;
+  launch_densify_and_prune(params, nullptr, nullptr, n, sh_k, active_mask, grad_accum, denom, max_radii, noise,
+                           densify_enabled, grad_threshold, min_opacity, extent, max_screen_size, workspace,
+                           info, (cudaStream_t)stream);
+  launch_moments8_move(mu, nu, mu_exp, nu_exp, n, sh_k, density_sources(workspace, n),
+                       (char*)workspace + density_workspace_bytes(n), (cudaStream_t)stream);
+  return last_error();
+}
+
 int gs_reset_opacities(float* params, int n, const uint8_t* active_mask, float reset_val, gs_stream_t stream) {
   if (n < 0 || (n > 0 && (!params || !active_mask))) return GS_ERR_INVALID_ARGUMENT;
   if (!(reset_val > 0.f && reset_val < 1.f)) return GS_ERR_INVALID_ARGUMENT;

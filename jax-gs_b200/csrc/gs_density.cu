@@ -213,7 +213,19 @@ k_dens_route(uint8_t* __restrict__ active, float* __restrict__ grad_accum, int* 
   denom[i] = 0;
 }
 
-// The moves, one warp each, over a persistent grid.
+// source[slot] = the row that moves there (-1 elsewhere, set before).
+__global__ void __launch_bounds__(256)
+k_dens_sources(const int2* __restrict__ moves, const int* __restrict__ info, int* __restrict__ source) {
+  GS_PDL_ENTRY_PLAIN();
+  const int total = info[1] + info[2];
+  for (int m = blockIdx.x * 256 + threadIdx.x; m < total; m += gridDim.x * 256) {
+    const int2 mv = moves[m];
+    source[mv.y < 0 ? -1 - mv.y : mv.y] = mv.x;
+  }
+}
+
+// The moves, one warp each, over a persistent grid. mu, nu NULL: moments in 8
+// bits, which move between blocks (launch_moments8_move).
 __global__ void __launch_bounds__(256)
 k_dens_copy(float* __restrict__ params, float* __restrict__ mu, float* __restrict__ nu,
             const int2* __restrict__ moves, const int* __restrict__ info, const float* __restrict__ noise,
@@ -229,8 +241,10 @@ k_dens_copy(float* __restrict__ params, float* __restrict__ mu, float* __restric
     const bool split = mv.y < 0;
     const int src = mv.x, dst = split ? -1 - mv.y : mv.y;
     warp_copy_row(params, n, w_sh, src, dst, lane);
-    warp_copy_row(mu, n, w_sh, src, dst, lane);
-    warp_copy_row(nu, n, w_sh, src, dst, lane);
+    if (mu) {
+      warp_copy_row(mu, n, w_sh, src, dst, lane);
+      warp_copy_row(nu, n, w_sh, src, dst, lane);
+    }
     __syncwarp();  // the source row is read before the split changes it
     if (split && lane < 3) {
       split_row(params, n, dst, a.log16, noise, lane);
@@ -295,6 +309,19 @@ void launch_densify_and_prune(float* params, float* mu, float* nu, int n, int sh
     grid = sms * (per_sm > 0 ? per_sm : 1);
   }
   launch_kernel_plain(k_dens_copy, grid, 256, 0, st, params, mu, nu, moves, info, noise, a);
+  if (!mu) {
+    // the list of empty slots has been read: its memory holds the map of the moved rows
+    cudaMemsetAsync(empty_list, 0xFF, (size_t)n * sizeof(int), st);
+    launch_kernel_plain(k_dens_sources, grid, 256, 0, st, moves, info, empty_list);
+  }
+}
+
+// The row that each slot received in launch_densify_and_prune without fp32
+// moments, -1 for none.
+const int* density_sources(const void* ws, int n) {
+  const size_t nb = (size_t)((n + 255) / 256);
+  auto al = [](size_t x) { return (x + 255) & ~(size_t)255; };
+  return (const int*)((const char*)ws + al((size_t)n) + al(4 * nb * sizeof(int)) + al(3 * nb * sizeof(int)));
 }
 
 void launch_reset_opacities(float* params, int n, const uint8_t* active, float reset_val, cudaStream_t st) {

@@ -208,6 +208,7 @@ void launch_densify_and_prune(float* params, float* mu, float* nu, int n, int sh
                               float* grad_accum, int* denom, const float* max_radii, const float* noise,
                               int enabled, float grad_threshold, float min_opacity, float extent,
                               float max_screen_size, void* ws, int* info, cudaStream_t st);
+const int* density_sources(const void* ws, int n);
 void launch_reset_opacities(float* params, int n, const uint8_t* active, float reset_val, cudaStream_t st);
 
 // gs_2dgs.cu: the 2DGS surfel renderer, regularisers and flat Adam.
@@ -267,6 +268,9 @@ void launch_moments8_decode(const uint8_t* mu, const uint8_t* nu, const uint8_t*
                             long long count, int type, void* mu_out, void* nu_out, cudaStream_t st);
 void launch_moments8_encode(const float* mu, const float* nu, long long count, uint8_t* mu8, uint8_t* nu8,
                             uint8_t* mu_exp, uint8_t* nu_exp, cudaStream_t st);
+size_t moments8_move_bytes(int n, int sh_k);
+void launch_moments8_move(uint8_t* mu, uint8_t* nu, uint8_t* mu_exp, uint8_t* nu_exp, int n, int sh_k,
+                          const int* source, void* ws, cudaStream_t st);
 
 // gs_ssim.cu
 size_t dssim_workspace_bytes(int h, int w, int c);

@@ -2,7 +2,8 @@
 
 DensityState and init_density_state live in trainer.py (flat buffers);
 densify_and_prune and reset_opacities update a state in place on the device
-(gs_densify_and_prune, gs_reset_opacities) and return it, like the
+(gs_densify_and_prune or, with 8-bit moments, gs_densify_and_prune8;
+gs_reset_opacities) and return it, like the
 reference's functional versions return a new state.
 
 Data parallel (train_parallel.py:269-283): densify_and_prune_parallel runs
@@ -51,26 +52,24 @@ def densify_and_prune(state: DensityState, rng_key: Union[int, torch.Generator, 
     if noise.shape != (state.n, 3):
         raise ValueError(f"noise must have shape ({state.n}, 3)")
     b = state._buffers.setdefault("density", {})
-    if "ws" not in b:
-        b["ws"] = torch.empty(max(256, _lib.lib().gs_density_workspace_bytes(state.n)), dtype=torch.uint8,
-                              device=dev)
+    m8 = state.moments8
+    if "info" not in b:
         b["info"] = torch.zeros(4, dtype=torch.int32, device=dev)
+        if m8 is None:
+            b["ws"] = torch.empty(max(256, _lib.lib().gs_density_workspace_bytes(state.n)), dtype=torch.uint8,
+                                  device=dev)
+    # with 8-bit moments the workspace holds a copy of one moment's codes: given back after the call
+    if m8 is None:
+        ws = b["ws"]
+    else:
+        ws = torch.empty(max(256, _lib.lib().gs_density8_workspace_bytes(state.n, state.sh_k)), dtype=torch.uint8,
+                         device=dev)
     P = _lib.ptr
-    mu, nu = state.mu, state.nu
-    if state.moments8 is not None:
-        # 8-bit moments move between blocks with other exponents: as values,
-        # rounded to nearest where a block has changed
-        flat = state.moments8.values()
-        mu, nu = (torch.cat(state.moments8.split(t)) for t in flat)
-    _lib.call("gs_densify_and_prune", P(state.params), P(mu), P(nu), state.n, state.sh_k,
+    _lib.call("gs_densify_and_prune" if m8 is None else "gs_densify_and_prune8", P(state.params),
+              *(P(t) for t in state.moment_buffers()), state.n, state.sh_k,
               P(state.active_mask.view(torch.uint8)), P(state.grad_accum), P(state.denom), P(state.max_radii),
               P(noise), int(bool(densify_enabled)), float(grad_threshold), float(min_opacity), float(extent),
-              float(max_screen_size), P(b["ws"]), b["ws"].numel(), P(b["info"]), _lib.stream(dev))
-    if state.moments8 is not None:
-        for t, moved in zip(flat, (mu, nu)):
-            for part, (lo, hi) in zip(state.moments8.split(t), state.segments):
-                part.copy_(moved[lo:hi])
-        state.moments8.set_values(*flat)
+              float(max_screen_size), P(ws), ws.numel(), P(b["info"]), _lib.stream(dev))
     state.densify_info = b["info"]
     return state
 
