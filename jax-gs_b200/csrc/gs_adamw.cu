@@ -8,8 +8,9 @@
 //   p' = p - lr (m' / (1 - b1^t) / (sqrt(v' / (1 - b2^t)) + eps) + wd p)
 // in fp32 throughout; m' and v' are sums of two rounded products (no FMA), so
 // that the 8-bit codes are a function of the inputs that any fp32
-// implementation reproduces bit for bit (but the sign of a zero). p' needs no such care: its divide
-// and square root are the approximate ones (a few ulps of the update).
+// implementation reproduces bit for bit (but the sign of a zero). p' takes a
+// root and a quotient that are rounded to nearest; only the kernel for many
+// elements with 8-bit moments takes the approximate ones (adamw_param4_fast).
 //
 // 8-bit moments. A block is 128 elements, counted from the tensor's start.
 // Each moment has one exponent byte a block,
@@ -193,13 +194,49 @@ struct AdamwStep {
   float rate, decay;  // lr inv1 and -lr wd of the tensor
 };
 
-// p - lr (m inv1 / (sqrt(v inv2) + eps) + wd p) for four elements. eps is a
-// normal float, so the denominator is one too and lies far below 2^126: the
-// approximate reciprocal needs no care for subnormals. The root of a
-// subnormal is below 2^-63; as 0 it changes a denominator by less than a
-// rounding unless eps < 2^-39.
+// p - lr (m inv1 / (sqrt(v inv2) + eps) + wd p) for four elements, root and
+// quotient to nearest but for rare ties: the approximations and one Newton step
+// each. x = v inv2 that overflowed stays an infinite denominator (x 2^-126 is
+// below 2^-62 of the root of any other x), clamped to a number whose
+// approximate reciprocal is 0; NaN passes. The root of a subnormal x is below
+// 2^-63 and comes out anywhere below that, which changes a denominator by less
+// than a rounding unless eps < 2^-39: then the compiler's root and quotient.
+// 32-bit moments, bound by memory: 59M elements 260 us, 259 with the
+// approximations alone, 273 with the compiler's; 12M, half of them off: 45.5,
+// 45.2, 60.
 __device__ __forceinline__ void adamw_param4(const float p[4], const float m[4], const float v[4], const AdamwStep& h,
                                              const AdamwParams& a, float out[4]) {
+  constexpr float kMost = 3.402823466e38f, kLeast = 0x1p-126f;
+  if (a.fine_root) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      out[q] = fmaf(h.decay, p[q], p[q]) - __fdiv_rn(m[q] * h.rate, __fsqrt_rn(v[q] * h.inv2) + a.eps);
+    return;
+  }
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    const float x = v[q] * h.inv2, n = m[q] * h.rate;
+    float xc, y, den, r;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(xc) : "f"(x), "f"(kMost));
+    asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(fmaxf(xc, kLeast)));
+    const float s = xc * y;
+    const float root = fmaf(fmaf(-s, s, xc), 0.5f * y, s);
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(den) : "f"(root + fmaf(x, kLeast, a.eps)), "f"(kMost));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(den));
+    const float t = n * r;
+    out[q] = fmaf(h.decay, p[q], p[q]) - fmaf(fmaf(-t, den, n), r, t);
+  }
+}
+
+// The same with the approximate root and reciprocal (2^-23 of each at most):
+// the update is off by up to 4 units of 2^-24 instead of 2, below its own
+// uncertainty from moments of 4 significant bits. For k_adamw8, which is bound
+// by the issue of instructions: 236M elements 575 us so, 626 with the Newton
+// steps, 955 with the compiler's root and quotient. eps is a normal float, so
+// the denominator is one too and lies far below 2^126: the approximate
+// reciprocal needs no care for subnormals.
+__device__ __forceinline__ void adamw_param4_fast(const float p[4], const float m[4], const float v[4],
+                                                  const AdamwStep& h, const AdamwParams& a, float out[4]) {
   float root[4];
   if (a.fine_root) {
 #pragma unroll
@@ -915,7 +952,7 @@ __device__ __forceinline__ void adamw8_blocks(const AdamwDesc& d, const Adamw8Ch
     }
     if (ALL || COPY || c.kind != kNone) {
       load4<true>(st.p, e, p);
-      adamw_param4(p, m + 4 * i, v + 4 * i, h, a, fresh);
+      adamw_param4_fast(p, m + 4 * i, v + 4 * i, h, a, fresh);
       if (!ALL) {
 #pragma unroll
         for (int q = 0; q < 4; ++q)
