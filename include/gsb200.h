@@ -548,8 +548,9 @@ GS_API int gs_adam_step_flat_device(float* params, const float* grads, float* mu
 /*
  * No reference counterpart (the reference's optimizers are optax.adam over
  * fixed groups): AdamW with decoupled weight decay as optax.adamw defines it,
- * over any number of tensors of any sizes in one launch per 256 of them (128
- * where the alignment of each differs).
+ * over any number of tensors of any sizes in one launch per 256 of them (with
+ * moments in 32 bits, tensors of which all arrays lie the same 1 to 3 elements
+ * behind a 16-byte boundary, for 16-bit values an 8-byte one, count twice).
  * With c = state[0] before the call, t = c + 1 and s = *grad_scale (1 if
  * NULL), for every element of every tensor:
  *   g  = s grad;  m' = b1 m + (1 - b1) g;  v' = b2 v + (1 - b2) g^2
@@ -610,6 +611,10 @@ typedef struct GsAdamwConfig {
  * index of the tensor, block, element) for each moment; nu' > 0 never becomes
  * 0. The sign of a zero mu is not specified. The parameter's update uses the
  * new moments before they are rounded.
+ *
+ * The update's root and quotient are rounded to nearest in fp32 (all but a few
+ * near ties); with 8-bit moments and many elements (more than 4096 per SM) they
+ * are approximations, 2^-23 off at most.
  */
 GS_API int gs_adamw_step(const GsAdamwTensor* tensors, int n_tensors, const GsAdamwConfig* config,
                          const float* grad_scale, int32_t* state, gs_stream_t stream);

@@ -32,8 +32,8 @@
 // Bytes an element with fp32 gradients: 28 with 32-bit moments, 16 with 8-bit
 // ones. Measured on a B200 whose copies run at 6.45 TB/s: the 32-bit step on
 // 59M elements 260 us (28 B: 6.35 TB/s, bound by HBM); the 8-bit step on 236M
-// elements, a quarter of them in rows that are off, 572 us (13.5 B moved:
-// 5.6 TB/s), bound by HBM and by the issue of 62 instructions an element
+// elements, a quarter of them in rows that are off, 576 us (13.5 B moved:
+// 5.5 TB/s), bound by HBM and by the issue of 62 instructions an element
 // (2.7 of 4 a cycle); the norm of 236M fp32 gradients 141 us (6.7 TB/s, some
 // of it from L2).
 #include <algorithm>
@@ -106,7 +106,9 @@ struct AdamwDesc {
 // AdamwDesc::vec: accesses of one element, of four, and (8-bit moments, fp32
 // gradients) of four but for the parameter and the gradient, which are not
 // 16-byte aligned: they pass through shared memory word by word (59M elements:
-// 200 us, aligned 160).
+// 201 us, aligned 161). 8-bit moments with 16-bit gradients off the alignment
+// are kScalar, element by element (59M: 777 us, aligned 158), as are 32-bit
+// ones whose arrays lie differently far behind it (275 us, aligned 258).
 constexpr int kScalar = 0, kVec = 1, kLoose = 2;
 
 // Tables travel as kernel parameters (no device copy, nothing to keep alive,
@@ -788,7 +790,7 @@ k_adamw_small(const __grid_constant__ AdamwTable<N> tab, const __grid_constant__
 
 // 8-bit moments. The step's instructions take the SMs about as long as its
 // bytes take the memory (the same step with a block a warp and every test at
-// each element: 98 instructions, 765 us at 236M elements, now 62 and 572), so
+// each element: 98 instructions, 765 us at 236M elements, now 62 and 576), so
 //  - no warp waits for memory: each copies its next chunk into shared memory
 //    (cp.async, 16 bytes a lane) before it works on the current one;
 //  - half a warp holds a block, eight elements a lane in two groups of four,
@@ -1328,7 +1330,7 @@ k_grad_norm(const __grid_constant__ GradTable<N> tab, double* __restrict__ parti
   const int tiles = tab.first[tab.n];
   // Many tensors: consecutive tiles, so that a CTA reads few entries of the
   // table (each new one is a miss of the constant cache: 197 tensors of 100 MB
-  // took 39 us in strides and 26 us so). Few: strides, which end more evenly.
+  // took 39 us in strides and 28 us so). Few: strides, which end more evenly.
   constexpr bool kRange = N > kNormSmall;
   const int t0 = kRange ? (int)((long long)tiles * blockIdx.x / gridDim.x) : (int)blockIdx.x;
   const int t1 = kRange ? (int)((long long)tiles * (blockIdx.x + 1) / gridDim.x) : tiles;
@@ -1424,7 +1426,8 @@ void launch_grad_norm(const GsGradTensor* tensors, int n, float max_norm, const 
 // ---------------------------------------------------------------------------
 // 8-bit moments to and from values. Encoding rounds to nearest (halves up):
 // the values of a block's codes are kept exactly. Decoding 236M elements to
-// bf16: 245 us (6 B an element: 5.8 TB/s).
+// bf16: 245 us (6 B an element: 5.8 TB/s); encoding them from fp32: 521 us
+// (10 B: 4.5 TB/s, a byte a lane).
 __device__ __forceinline__ void store_value(float* p, float x) { *p = x; }
 __device__ __forceinline__ void store_value(__nv_bfloat16* p, float x) { *p = __float2bfloat16_rn(x); }
 
@@ -1570,8 +1573,9 @@ void launch_moments8_encode(const float* mu, const float* nu, long long count, u
 // rows is encoded again as a whole, to nearest; the others are not touched.
 // Values are read from a copy of the codes: a source may lie in a block that
 // is encoded again. 240k of 4M rows moved (236M elements):
-// both moments 1.35 ms, of which the copies are 0.2; the rest are the tests of
-// every element's row, and it runs once in a hundred steps.
+// both moments 1.35 ms, 0.15 of it the copies at the rate of a copy, the rest
+// the tests of every element's row and the blocks encoded again. A training
+// runs it once in a hundred steps.
 struct Moments8Groups {
   int first[6];    // first block of each group
   unsigned width[5];
