@@ -196,9 +196,9 @@ struct AdamwStep {
   float rate, decay;  // lr inv1 and -lr wd of the tensor
 };
 
-// p - lr (m inv1 / (sqrt(v inv2) + eps) + wd p) for four elements, root and
-// quotient to nearest but for rare ties: the approximations and one Newton step
-// each. x = v inv2 that overflowed stays an infinite denominator (x 2^-126 is
+// p - lr (m inv1 / (sqrt(v inv2) + eps) + wd p) for four elements, with one
+// rounding of p's own size: the decay joins the update, not p. Root and quotient
+// are to nearest but for rare ties: the approximations and one Newton step each. x = v inv2 that overflowed stays an infinite denominator (x 2^-126 is
 // below 2^-62 of the root of any other x), clamped to a number whose
 // approximate reciprocal is 0; NaN passes. The root of a subnormal x is below
 // 2^-63 and comes out anywhere below that, which changes a denominator by less
@@ -212,7 +212,7 @@ __device__ __forceinline__ void adamw_param4(const float p[4], const float m[4],
   if (a.fine_root) {
 #pragma unroll
     for (int q = 0; q < 4; ++q)
-      out[q] = fmaf(h.decay, p[q], p[q]) - __fdiv_rn(m[q] * h.rate, __fsqrt_rn(v[q] * h.inv2) + a.eps);
+      out[q] = p[q] + fmaf(h.decay, p[q], -__fdiv_rn(m[q] * h.rate, __fsqrt_rn(v[q] * h.inv2) + a.eps));
     return;
   }
 #pragma unroll
@@ -226,7 +226,7 @@ __device__ __forceinline__ void adamw_param4(const float p[4], const float m[4],
     asm("min.NaN.f32 %0, %1, %2;" : "=f"(den) : "f"(root + fmaf(x, kLeast, a.eps)), "f"(kMost));
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(den));
     const float t = n * r;
-    out[q] = fmaf(h.decay, p[q], p[q]) - fmaf(fmaf(-t, den, n), r, t);
+    out[q] = p[q] + fmaf(h.decay, p[q], -fmaf(fmaf(-t, den, n), r, t));
   }
 }
 
@@ -251,7 +251,7 @@ __device__ __forceinline__ void adamw_param4_fast(const float p[4], const float 
   for (int q = 0; q < 4; ++q) {
     float inv;
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(root[q] + a.eps));
-    out[q] = fmaf(-(m[q] * h.rate), inv, fmaf(h.decay, p[q], p[q]));
+    out[q] = p[q] + fmaf(-(m[q] * h.rate), inv, h.decay * p[q]);
   }
 }
 

@@ -5,6 +5,8 @@ import numpy as np
 import pytest
 import torch
 
+from tests import adamw_ref as R
+
 pytestmark = pytest.mark.gpu
 
 U = 2.0 ** -24
@@ -93,3 +95,26 @@ def test_values_at_the_ends(n, eps):
             root = float(np.sqrt(np.float64(np.float32(x) * np.float32(x))))
             want = -2.0 ** -7 * float(np.float32(x)) / (root + e)
             np.testing.assert_allclose(got, want, rtol=5 * U, atol=0)
+
+
+@pytest.mark.parametrize("bits,n,align", [(32, 5000, 0), (32, 900_000, 0), (32, 900_000, 1), (8, 5000, 0),
+                                          (8, 900_000, 0), (8, 900_000, 1)])
+@pytest.mark.parametrize("eps", [1e-8, 1e-15])
+def test_one_rounding_of_the_parameter(bits, n, align, eps):
+    """With weight decay too, p' is rounded once at its own size (2^-24 of it); the rest are roundings of the update
+    and of the decay, as tests/adamw_ref.py counts them."""
+    from gs_b200.training.optimizer import AdamW, ParamTensor
+    rng = np.random.default_rng(bits + n)
+    p0 = rng.standard_normal(n).astype(np.float32)
+    p = torch.zeros(n + align, device="cuda")[align:]
+    g = torch.zeros(n + align, device="cuda")[align:]
+    p.copy_(torch.tensor(p0))
+    g.copy_(torch.tensor(_gradient(n, -6, 0, 5)))
+    lr, wd = 1e-3, 0.3
+    AdamW([ParamTensor(p, g, lr=lr, weight_decay=wd)], eps=eps, moment_bits=bits).step()
+    z = np.zeros(n, np.float32)
+    m, v = R.moments(z, z, g.cpu().numpy(), 1.0, 0.9, 0.999)
+    want, _ = R.param(p0, m, v, 0, lr, wd, 0.9, 0.999, eps)
+    upd = np.abs(want - p0) + 2 * lr * wd * np.abs(p0)  # no less than the update and the decay apart
+    off = np.abs(p.cpu().numpy() - want) > U * np.abs(want) + 56 * U * upd
+    assert not off.any(), (int(off.sum()), np.flatnonzero(off)[:5])
