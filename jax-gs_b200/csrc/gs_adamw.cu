@@ -198,7 +198,8 @@ struct AdamwStep {
 
 // p - lr (m inv1 / (sqrt(v inv2) + eps) + wd p) for four elements, with one
 // rounding of p's own size: the decay joins the update, not p. Root and quotient
-// are to nearest but for rare ties: the approximations and one Newton step each. x = v inv2 that overflowed stays an infinite denominator (x 2^-126 is
+// are to nearest but for a few near ties: the approximations and one Newton step
+// each. x = v inv2 that overflowed stays an infinite denominator (x 2^-126 is
 // below 2^-62 of the root of any other x), clamped to a number whose
 // approximate reciprocal is 0; NaN passes. The root of a subnormal x is below
 // 2^-63 and comes out anywhere below that, which changes a denominator by less
@@ -1572,10 +1573,10 @@ void launch_moments8_encode(const float* mu, const float* nu, long long count, u
 // moment. A row's new block has another exponent, so a block that receives
 // rows is encoded again as a whole, to nearest; the others are not touched.
 // Values are read from a copy of the codes: a source may lie in a block that
-// is encoded again. 240k of 4M rows moved (236M elements):
-// both moments 1.35 ms, 0.15 of it the copies at the rate of a copy, the rest
-// the tests of every element's row and the blocks encoded again. A training
-// runs it once in a hundred steps.
+// is encoded again. 240k of 4M rows moved (236M elements): both moments 1.35 ms,
+// 0.15 of it the copies at the rate of a copy, the rest the tests of every
+// element's row and the blocks encoded again. A training runs it once in a
+// hundred steps.
 struct Moments8Groups {
   int first[6];    // first block of each group
   unsigned width[5];

@@ -385,8 +385,8 @@ void launch_step_stats(const float* grad_means, const float* means, const float*
   const float focal = (float)(((double)fx + (double)fy) / 2.0);
   const float pix3 = (float)((double)width * (double)height * 3.0);
   GS_TIMED("step_stats", st);
-  launch_kernel_plain(k_step_stats, nb, 256, 0, st, grad_means, means, w2c, n, focal, pix3, radii, valid, active, gate, grad_accum,
-                                    denom, max_radii, grad2d);
+  launch_kernel_plain(k_step_stats, nb, 256, 0, st, grad_means, means, w2c, n, focal, pix3, radii, valid, active, gate,
+                      grad_accum, denom, max_radii, grad2d);
 }
 
 void launch_density_stats(const float* grad2d, const float* radii, const uint8_t* valid,
@@ -396,7 +396,7 @@ void launch_density_stats(const float* grad2d, const float* radii, const uint8_t
   if (nb == 0) return;
   GS_TIMED("density_stats", st);
   launch_kernel_plain(k_density_stats, nb, 256, 0, st, grad2d, radii, valid, radii_valid, active, n, gate, grad_accum,
-                                       denom, max_radii);
+                      denom, max_radii);
 }
 
 }  // namespace gs

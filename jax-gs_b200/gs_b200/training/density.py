@@ -3,8 +3,8 @@
 DensityState and init_density_state live in trainer.py (flat buffers);
 densify_and_prune and reset_opacities update a state in place on the device
 (gs_densify_and_prune or, with 8-bit moments, gs_densify_and_prune8;
-gs_reset_opacities) and return it, like the
-reference's functional versions return a new state.
+gs_reset_opacities) and return it, like the reference's functional versions
+return a new state.
 
 Data parallel (train_parallel.py:269-283): densify_and_prune_parallel runs
 the density step on rank 0's state alone -- the reference's authoritative
